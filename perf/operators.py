@@ -283,8 +283,9 @@ def _plain_distill(s):
     scale = c["temperature"]
     r = {"loss": torch.where(live, loss * (scale * scale), 0.0).float()}
     if "d_loss" in s:
-        share = (q.sum(-1) + rest)[:, None]
+        share = q.sum(-1)[:, None]
         if c["tail"]:
+            share = share + torch.where(has, rest, 0.0)[:, None]
             shift = torch.where(has, rest / out, 0.0)[:, None]
             factor = torch.where(named, share.float(),
                                  (share - shift).float())
