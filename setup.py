@@ -21,7 +21,9 @@ common = dict(
     library_dirs=[rocm_lib],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
-        "nvcc": ["-O3", "-std=c++17"],
+        # no packed fp32 arithmetic: some of its forms are not reliable here
+        "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
+                 "-Xclang", "-packed-fp32-ops"],
     },
 )
 
@@ -35,7 +37,11 @@ ext_modules = [
     CUDAExtension(
         name="dear_pytorch_amd._kernels",
         sources=["dear_pytorch_amd/csrc/kernels.hip",
-                 "dear_pytorch_amd/csrc/bn_kernels.hip"],
+                 "dear_pytorch_amd/csrc/bn_kernels.hip",
+                 "dear_pytorch_amd/csrc/layer_norm.hip",
+                 "dear_pytorch_amd/csrc/token_loss.hip",
+                 "dear_pytorch_amd/csrc/lm_ops.cpp"],
+        depends=["dear_pytorch_amd/csrc/lm_common.h"],
         libraries=["amdhip64"],
         **common,
     ),
