@@ -434,6 +434,8 @@ static void bn_bwd(at::Tensor x, at::Tensor dy, at::Tensor y,
   HIP_CHECK(hipGetLastError());
 }
 
+void register_lm_ops(pybind11::module& m);   // lm_ops.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "DeAR CDNA4 fused kernels (gfx950)";
   m.def("bn_nparts", [](int64_t rows, int64_t C) {
@@ -448,4 +450,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("unpack_scale", &unpack_scale);
   m.def("count_ge", &count_ge);
   m.def("select_ge", &select_ge);
+  register_lm_ops(m);
 }
