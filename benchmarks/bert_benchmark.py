@@ -35,6 +35,14 @@ def main():
     p.add_argument("--amp", action="store_true",
                    help="bf16 autocast compute (reference --fp16 axis; "
                         "gradients/optimizer stay fp32)")
+    p.add_argument("--fused-ln", action="store_true",
+                   help="residual add + layer norm in one kernel")
+    p.add_argument("--fused-loss", action="store_true",
+                   help="masked-token loss over the labelled tokens only")
+    p.add_argument("--distill-top", type=int, default=0,
+                   help="learn from this many alternatives of a frozen "
+                        "bert_large as well (0: no teacher)")
+    p.add_argument("--distill-temperature", type=float, default=1.0)
     args = p.parse_args()
 
     import dear_pytorch_amd as dear
@@ -53,8 +61,20 @@ def main():
 
     cfg = models.bert_large() if args.model == "bert_large" else \
         models.bert_base()
+    cfg.fused_ln = args.fused_ln
     model = models.BertForPreTraining(cfg).to(device)
-    crit = models.BertPretrainingCriterion(cfg.vocab_size).to(device)
+    teacher = None
+    if args.distill_top:
+        big = models.bert_large()
+        big.fused_ln = args.fused_ln
+        teacher = models.BertForPreTraining(big).to(device).eval() \
+            .requires_grad_(False)
+        crit = models.BertDistillationCriterion(
+            cfg.vocab_size, top=args.distill_top,
+            temperature=args.distill_temperature).to(device)
+    else:
+        crit = models.BertPretrainingCriterion(
+            cfg.vocab_size, fused=args.fused_loss).to(device)
 
     bs, S = args.batch_size, args.sentence_len
     g = torch.Generator().manual_seed(77 + rank)
@@ -69,6 +89,8 @@ def main():
 
     if world > 1:
         dear.broadcast_parameters(model.state_dict(), root_rank=0)
+        if teacher is not None:
+            dear.broadcast_parameters(teacher.state_dict(), root_rank=0)
     base_opt = torch.optim.SGD(model.parameters(), lr=2e-5) \
         if args.optimizer == "sgd" else \
         torch.optim.AdamW(model.parameters(), lr=1e-4)
@@ -106,7 +128,12 @@ def main():
         opt.zero_grad()
         with amp_ctx():
             scores, seq_rel = model(ids, tt, mask)
-            loss = crit(scores, seq_rel, mlm, nsp)
+            if teacher is None:
+                loss = crit(scores, seq_rel, mlm, nsp)
+            else:
+                with torch.no_grad():
+                    said = crit.answers(teacher(ids, tt, mask)[0], mlm)
+                loss = crit(scores, seq_rel, mlm, nsp, said)
         loss.backward()
         opt.step()
         if tuner:

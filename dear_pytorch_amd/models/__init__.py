@@ -2,7 +2,7 @@
 + local inceptionv4 + transformers BERT; all are self-contained here)."""
 from . import resnet, vgg, densenet, inceptionv4 as _iv4, bert, mnist
 from .bert import (BertConfig, BertForPreTraining, BertPretrainingCriterion,
-                   bert_base, bert_large)
+                   BertDistillationCriterion, bert_base, bert_large)
 from .mnist import MnistNet
 
 _REGISTRY = {

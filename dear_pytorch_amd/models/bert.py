@@ -5,15 +5,24 @@ Capability parity with the reference's BERT benchmark path
 from bert_config.json + BertPretrainingCriterion).  Configs: Base 12L/768h/12
 heads, Large 24L/1024h/16 heads, vocab padded to a multiple of 8 (30528).
 Attention runs through torch.nn.functional.scaled_dot_product_attention
-(MIOpen/CK fused path on ROCm)."""
+(MIOpen/CK fused path on ROCm).
+
+BertConfig(fused_ln=True) takes ops/fused_ln.py for every layer norm, with the
+residual add in it; BertPretrainingCriterion(fused=True) takes the masked-token
+loss from ops/token_loss.py, and BertDistillationCriterion adds what a teacher
+says to it.  State dicts are the same either way."""
 from dataclasses import dataclass
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..ops.fused_ln import FusedLayerNorm
+from ..ops.token_loss import (TokenLogProbs, token_logprobs,
+                              topk_distill_loss)
+
 __all__ = ["BertConfig", "BertForPreTraining", "BertPretrainingCriterion",
-           "bert_base", "bert_large"]
+           "BertDistillationCriterion", "bert_base", "bert_large"]
 
 
 @dataclass
@@ -28,6 +37,19 @@ class BertConfig:
     hidden_dropout_prob: float = 0.1
     attention_probs_dropout_prob: float = 0.1
     layer_norm_eps: float = 1e-12
+    fused_ln: bool = False           # residual add + layer norm in one kernel
+
+
+def _layer_norm(c: BertConfig):
+    kind = FusedLayerNorm if c.fused_ln else nn.LayerNorm
+    return kind(c.hidden_size, eps=c.layer_norm_eps)
+
+
+def _add_norm(ln, x, h):
+    """ln(x + h), the residual add inside of the kernel where it can be."""
+    if isinstance(ln, FusedLayerNorm):
+        return ln(h, residual=x)
+    return ln(x + h)
 
 
 def bert_base():
@@ -45,7 +67,7 @@ class BertEmbeddings(nn.Module):
         self.word = nn.Embedding(c.vocab_size, c.hidden_size)
         self.position = nn.Embedding(c.max_position_embeddings, c.hidden_size)
         self.token_type = nn.Embedding(c.type_vocab_size, c.hidden_size)
-        self.ln = nn.LayerNorm(c.hidden_size, eps=c.layer_norm_eps)
+        self.ln = _layer_norm(c)
         self.drop = nn.Dropout(c.hidden_dropout_prob)
         self.register_buffer("pos_ids",
                              torch.arange(c.max_position_embeddings)[None],
@@ -81,16 +103,16 @@ class BertLayer(nn.Module):
     def __init__(self, c: BertConfig):
         super().__init__()
         self.attn = BertSelfAttention(c)
-        self.ln1 = nn.LayerNorm(c.hidden_size, eps=c.layer_norm_eps)
+        self.ln1 = _layer_norm(c)
         self.fc1 = nn.Linear(c.hidden_size, c.intermediate_size)
         self.fc2 = nn.Linear(c.intermediate_size, c.hidden_size)
-        self.ln2 = nn.LayerNorm(c.hidden_size, eps=c.layer_norm_eps)
+        self.ln2 = _layer_norm(c)
         self.drop = nn.Dropout(c.hidden_dropout_prob)
 
     def forward(self, x, attn_mask):
-        x = self.ln1(x + self.drop(self.attn(x, attn_mask)))
+        x = _add_norm(self.ln1, x, self.drop(self.attn(x, attn_mask)))
         h = self.fc2(F.gelu(self.fc1(x)))
-        return self.ln2(x + self.drop(h))
+        return _add_norm(self.ln2, x, self.drop(h))
 
 
 class BertModel(nn.Module):
@@ -119,7 +141,7 @@ class BertForPreTraining(nn.Module):
         self.config = c
         self.bert = BertModel(c)
         self.transform = nn.Linear(c.hidden_size, c.hidden_size)
-        self.transform_ln = nn.LayerNorm(c.hidden_size, eps=c.layer_norm_eps)
+        self.transform_ln = _layer_norm(c)
         self.decoder = nn.Linear(c.hidden_size, c.vocab_size, bias=True)
         self.decoder.weight = self.bert.embeddings.word.weight  # tied
         self.nsp = nn.Linear(c.hidden_size, 2)
@@ -138,15 +160,66 @@ class BertForPreTraining(nn.Module):
 
 
 class BertPretrainingCriterion(nn.Module):
-    """MLM + NSP cross-entropy (reference dear/bert_benchmark.py:101-112)."""
+    """MLM + NSP cross-entropy (reference dear/bert_benchmark.py:101-112).
 
-    def __init__(self, vocab_size):
+    fused=True takes the MLM part from token_logprobs, which reads the logits
+    of labelled tokens only."""
+
+    def __init__(self, vocab_size, fused=False):
         super().__init__()
         self.vocab_size = vocab_size
+        self.fused = fused
         self.ce = nn.CrossEntropyLoss(ignore_index=-1)
 
+    def masked_token_loss(self, pred_scores, mlm_labels):
+        """Mean over the labelled tokens; NaN where there is none, as
+        nn.CrossEntropyLoss gives it."""
+        scores = pred_scores.view(-1, self.vocab_size)
+        labels = mlm_labels.view(-1)
+        if not self.fused:
+            return self.ce(scores, labels)
+        lp = token_logprobs(scores, labels, ignore_index=-1).logprob
+        return -lp.sum() / (labels != -1).sum()
+
     def forward(self, pred_scores, nsp_scores, mlm_labels, nsp_labels):
-        mlm = self.ce(pred_scores.view(-1, self.vocab_size),
-                      mlm_labels.view(-1))
+        mlm = self.masked_token_loss(pred_scores, mlm_labels)
         nsp = self.ce(nsp_scores.view(-1, 2), nsp_labels.view(-1))
         return mlm + nsp
+
+
+class BertDistillationCriterion(BertPretrainingCriterion):
+    """The pretraining loss of a student with a teacher's answers in it:
+
+        (1 - weight) * MLM + weight * distillation + NSP
+
+    The distillation part is the mean of topk_distill_loss over the labelled
+    tokens, from the teacher's ``top`` alternatives at ``temperature``; with
+    ``tail`` the rest of the vocabulary counts as one more alternative.
+    """
+
+    def __init__(self, vocab_size, top=32, temperature=1.0, weight=0.5,
+                 tail=True):
+        super().__init__(vocab_size, fused=True)
+        if not 0.0 <= weight <= 1.0:
+            raise ValueError(f"weight must be 0 to 1, got {weight}")
+        if not 1 <= top <= vocab_size:
+            raise ValueError(f"top must be 1 to the vocabulary, got {top}")
+        self.top, self.temperature = top, temperature
+        self.weight, self.tail = weight, tail
+
+    @torch.no_grad()
+    def answers(self, teacher_scores, mlm_labels) -> TokenLogProbs:
+        """What the teacher says about the labelled tokens: this, not its
+        logits, is kept or sent until the student's step."""
+        return token_logprobs(teacher_scores, mlm_labels, top=self.top,
+                              temperature=self.temperature, ignore_index=-1)
+
+    def forward(self, pred_scores, nsp_scores, mlm_labels, nsp_labels,
+                answers: TokenLogProbs):
+        loss = topk_distill_loss(
+            pred_scores, answers.top_ids, answers.top_logprobs,
+            temperature=self.temperature, tail=self.tail)
+        learned = loss.sum() / (mlm_labels != -1).sum()
+        mlm = self.masked_token_loss(pred_scores, mlm_labels)
+        nsp = self.ce(nsp_scores.view(-1, 2), nsp_labels.view(-1))
+        return (1.0 - self.weight) * mlm + self.weight * learned + nsp
