@@ -37,14 +37,85 @@ __device__ __forceinline__ void store_as(void* p, int type, int64_t i,
   else static_cast<f16*>(p)[i] = static_cast<f16>(v);
 }
 
+// ------------------------------------------------- 16 bytes of a row at once
+using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
+
+template <typename T>
+constexpr int kVec = 16 / (int)sizeof(T);
+
+// Aligned to the element only: gfx950 loads and stores 16 bytes at any
+// address, so that odd widths and strides need no kernel of their own.
+template <typename T>
+__device__ __forceinline__ u32x4 load16(const T* p) {
+  u32x4 v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void store16(T* p, u32x4 v) {
+  __builtin_memcpy(p, &v, 16);
+}
+
+// Element j (known when compiled) of 16 bytes, as fp32.
+template <typename T>
+__device__ __forceinline__ float elem(u32x4 v, int j) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(v[j]);
+  } else if constexpr (__is_same(T, bf16)) {
+    return __uint_as_float(j & 1 ? v[j >> 1] & 0xffff0000u : v[j >> 1] << 16);
+  } else {
+    return to_f(__builtin_bit_cast(f16, (uint16_t)(v[j >> 1] >> (j & 1) * 16)));
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void put(u32x4& v, int j, T x) {
+  if constexpr (sizeof(T) == 4) {
+    v[j] = __float_as_uint(x);
+  } else {
+    const uint32_t u = __builtin_bit_cast(uint16_t, x);
+    v[j >> 1] = j & 1 ? (v[j >> 1] & 0xffffu) | u << 16
+                      : (v[j >> 1] & 0xffff0000u) | u;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ u32x4 pack(const float* r) {
+  T t[kVec<T>];
+#pragma unroll
+  for (int j = 0; j < kVec<T>; ++j) t[j] = static_cast<T>(r[j]);
+  u32x4 v;
+  __builtin_memcpy(&v, t, 16);
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ u32x4 minus_inf() {
+  const uint32_t u = sizeof(T) == 4         ? 0xff800000u
+                     : __is_same(T, bf16) ? 0xff80ff80u
+                                          : 0xfc00fc00u;
+  return u32x4{u, u, u, u};
+}
+
+// A number that is part of a type, to choose a kernel's sizes with.
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
 struct Add {
   template <typename A>
   __device__ __forceinline__ A operator()(A a, A b) const { return a + b; }
 };
+struct Max {
+  __device__ __forceinline__ float operator()(float a, float b) const {
+    return fmaxf(a, b);
+  }
+};
 // NaN wins: a row that holds one has to say so
 struct MaxNan {
   __device__ __forceinline__ float operator()(float a, float b) const {
-    return (a > b || a != a) ? a : b;
+    return __builtin_elementwise_maximum(a, b);
   }
 };
 
@@ -65,6 +136,20 @@ __device__ __forceinline__ A block_reduce(A v, Op op, A* scratch) {
   v = scratch[0];
   for (int i = 1; i < waves; ++i) v = op(v, scratch[i]);
   __syncthreads();
+  return v;
+}
+
+// The block's maximum in every thread, NaN if there is one; NT / 64 is a power
+// of two. One barrier: `scratch` must not be written again before the next.
+template <int NT>
+__device__ __forceinline__ float block_max(float v, float* scratch) {
+  constexpr int W = NT / 64;
+  v = wave_reduce(v, MaxNan{});
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = scratch[threadIdx.x & (W - 1)];
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) v = MaxNan{}(v, __shfl_xor(v, o));
   return v;
 }
 

@@ -15,15 +15,17 @@ int dear_ln_bwd(hipStream_t, int, int, int, const void*, int64_t, const void*,
                 int64_t, const void*, int64_t, const void*, const float*,
                 const float*, void*, void*, void*, void*, float*, int, int64_t,
                 int);
+int64_t dear_logit_slices(int, int);
+int64_t dear_slice_bytes();
 int dear_logprobs_fwd(hipStream_t, int, const void*, int64_t, const int64_t*,
                       int64_t, int64_t, int, int, double, float*, float*,
-                      float*, int64_t*, void*);
+                      float*, int64_t*, void*, void*, void*);
 int dear_logprobs_bwd(hipStream_t, int, const void*, int64_t, const int64_t*,
                       const int64_t*, const void*, const float*, const float*,
                       const float*, void*, int64_t, int, int, double);
 int dear_distill_fwd(hipStream_t, int, bool, const void*, int64_t,
                      const int64_t*, const float*, int64_t, int, int, double,
-                     float*, float*, void*);
+                     float*, float*, void*, void*);
 int dear_distill_bwd(hipStream_t, int, const void*, int64_t, const int64_t*,
                      const float*, const void*, const float*, void*, int64_t,
                      int, int, double);
@@ -245,6 +247,14 @@ void check_logits(const Tensor& t, const char* name) {
                     "tokens");
 }
 
+// What the slices of rows leave for each other, where a row has more than one
+Tensor slice_records(const Tensor& logits, const LogitRows& z) {
+  const int64_t n = dear_logit_slices(type_code(logits, "logits"), z.width);
+  if (n == 1) return Tensor();
+  return at::empty({z.rows * n, dear_slice_bytes()},
+                   logits.options().dtype(at::kByte));
+}
+
 // logprob (where there are tokens), entropy, and with top > 0 the top's log
 // probabilities and ids
 variable_list logprobs_forward(const Tensor& logits, const Tensor& tokens,
@@ -265,11 +275,16 @@ variable_list logprobs_forward(const Tensor& logits, const Tensor& tokens,
   if (stats) *stats = at::empty({z.rows, 4}, fopt);
   if (z.rows) {
     const Tensor tok = tokens.defined() ? tokens.contiguous() : Tensor();
+    const int type = type_code(logits, "logits");
+    const Tensor part = slice_records(logits, z);
+    Tensor lists;
+    if (top && part.defined())
+      lists = at::empty({part.size(0), top}, logits.options().dtype(at::kLong));
     check_launch(dear_logprobs_fwd(
-        stream_of(logits), type_code(logits, "logits"), data(z.t),
+        stream_of(logits), type, data(z.t),
         z.t.dim() == 2 ? z.t.stride(0) : 0, idata(tok), ignore, z.rows,
         z.width, (int)top, t, fdata(lp), fdata(h), fdata(tlp), idata(tid),
-        stats ? data(*stats) : nullptr));
+        stats ? data(*stats) : nullptr, data(part), data(lists)));
   }
   variable_list out;
   if (tokens.defined()) out.push_back(lp);
@@ -366,11 +381,12 @@ Tensor distill_forward(const Tensor& logits, const Tensor& ids,
   if (z.rows) {
     const Tensor idc = ids.contiguous();
     const Tensor tc = teacher.to(at::kFloat).contiguous();
+    const Tensor part = slice_records(logits, z);
     check_launch(dear_distill_fwd(
         stream_of(logits), type_code(logits, "logits"), tail, data(z.t),
         z.t.dim() == 2 ? z.t.stride(0) : 0, idata(idc), fdata(tc), z.rows,
         z.width, (int)k, t, fdata(loss), q ? fdata(*q) : nullptr,
-        stats ? data(*stats) : nullptr));
+        stats ? data(*stats) : nullptr, data(part)));
   }
   return loss;
 }

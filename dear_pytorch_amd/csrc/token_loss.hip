@@ -13,10 +13,20 @@
 //   W = sum q_k + q_t. Where the student gives nothing to the tokens outside
 //   (p_t = 0) the term of q_t is left out of loss and W.
 //
-// Elements are fp32; the sums of a thread are fp32 and those over threads
-// fp64. s is 1 + r for a row that is sure of its token: the elements equal to
-// m are counted and the others are added up by themselves, so that
-// log s = log1p(r) keeps the digits of a probability near one.
+// Forward: a block takes a slice of one row into registers, 16 bytes a load,
+// and passes over it there: the maximum, then the sums, then the top. A
+// vocabulary of up to 32768 fp32 or 65536 16-bit tokens is one slice, and the
+// block finishes the row; longer rows leave a record for each slice, and a
+// second kernel joins them. Backward: one pass, elementwise, then the few
+// named tokens again.
+//
+// Precision: exp(t) is exp2((z - m) c) with c = log2(e) / T: the difference is
+// taken first, so that it is 0 for the largest element and small errors stay
+// small whatever the size of m. What c loses in fp32 is the same for all
+// elements and is taken out of the sum in fp64. Sums of a wave are fp32, those
+// over waves fp64. The elements equal to m are counted apart: s = 1 + r for a
+// row that is sure of its token, and log1p(r) keeps the digits of a
+// probability near one.
 #include <hip/hip_runtime.h>
 
 #include "lm_common.h"
@@ -25,345 +35,865 @@ namespace {
 
 using namespace dear_lm;
 
-constexpr int kThreads = 256;
+constexpr int kMaxTop = 128;          // entries of a row
 constexpr int kMaxBlocks = 1 << 20;   // a launch holds under 2^32 threads
-constexpr int kMaxTop = 128;          // entries of a row, a thread for each
-constexpr int kChunk = 1 << 16;       // tokens of one bitmap of named ones
+constexpr int kCandidates = 1024;     // of a slice's top, kept for ranking
 constexpr double kLn2 = 0.69314718055994530942;
 
 // A key that orders as the logits do: larger is better, NaN above all, both
-// zeros equal.
+// zeros equal. No logit has the key 0.
 __device__ __forceinline__ uint32_t order_key(float z) {
   if (z != z) return 0xffffffffu;
   const uint32_t u = __float_as_uint(z + 0.0f);
   return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-// What a row leaves for its backward pass. inv_s == 0: nothing, its gradient
-// is zero.
+// Key and id of an alternative in one word: no two are equal, and of equal
+// logits the lower id is the larger word.
+__device__ __forceinline__ uint64_t candidate(float z, int id) {
+  return (uint64_t)order_key(z) << 32 | ~(uint32_t)id;
+}
+__device__ __forceinline__ int id_of(uint64_t c) { return ~(uint32_t)c; }
+
+// What a row leaves for its backward pass: p_j = exp2((z_j - m) c) inv_s.
+// inv_s == 0: the row was not looked at, its gradient is zero.
 struct RowStats {
   float m, inv_s, a, b;
 };
 
-struct RowSums {
-  float m;
-  bool bad;         // the largest logit is not a number that can be a maximum
-  double log_s, s, e2, out;
+// log2(e) / T and what fp32 leaves of it.
+struct Factor {
+  float c;
+  double exact;
 };
 
-// Top of a row by bisection: the largest key that at least k elements reach,
-// then, among the elements equal to it, the lowest indices.
-template <typename T>
-__device__ void row_top(const T* z, int V, int k, uint64_t* found, int* count,
-                        int* scratch) {
+// The sums of a slice or of a row, relative to its maximum m: n elements are
+// equal to m, `rest` and e2 (of e log2 e) are over the others. With a tail
+// these are the elements outside, and n_in and in are over the named ones.
+struct Sums {
+  double m, n, rest, e2, n_in, in;
+};
+
+__device__ __forceinline__ bool no_distribution(float m) {
+  return !(fabsf(m) < INFINITY);
+}
+
+// ------------------------------------------------------- a slice in registers
+template <typename T, int NT, int NV>
+struct Slice {
+  static constexpr int E = kVec<T>;
+  static constexpr int kTokens = NT * NV * E;
+  u32x4 raw[NV];
+  float vmax[NV];
+
+  static __device__ __forceinline__ int first(int v) {
+    return (v * NT + (int)threadIdx.x) * E;
+  }
+  __device__ __forceinline__ float at(int v, int j) const {
+    return elem<T>(raw[v], j);
+  }
+  // tokens [0, len) of z; what lies behind is -inf, which adds nothing
+  __device__ __forceinline__ void load(const T* z, int len) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int i = first(v);
+      if (i + E <= len) {
+        raw[v] = load16(z + i);
+      } else {
+        raw[v] = minus_inf<T>();
+        for (int j = 0; j < E; ++j)
+          if (i + j < len) put(raw[v], j, z[i + j]);
+      }
+    }
+  }
+  // NaN if the thread holds one
+  __device__ __forceinline__ float max() {
+    float m = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float a = at(v, 0);
+#pragma unroll
+      for (int j = 1; j < E; ++j) a = __builtin_elementwise_maximum(a, at(v, j));
+      vmax[v] = a;
+      m = __builtin_elementwise_maximum(m, a);
+    }
+    return m;
+  }
+};
+
+// The lists of a slice's top, by bisection in memory: the largest key that at
+// least k elements reach, then, among the elements equal to it, the lowest
+// ids. For rows whose order the quick way cannot use: NaN, or very many equal
+// elements. 31 + 32 passes over the slice.
+template <typename T, int NT>
+__device__ void bisect_top(const T* z, int len, int base, int k,
+                           uint64_t* found, int* count, int* scratch) {
   uint32_t key = 0;
   for (int bit = 31; bit >= 0; --bit) {
     const uint32_t want = key | (1u << bit);
     int n = 0;
-    for (int i = threadIdx.x; i < V; i += kThreads)
+    for (int i = threadIdx.x; i < len; i += NT)
       n += order_key(to_f(z[i])) >= want;
     if (block_reduce(n, Add{}, scratch) >= k) key = want;
   }
   int above = 0;
-  for (int i = threadIdx.x; i < V; i += kThreads)
+  for (int i = threadIdx.x; i < len; i += NT)
     above += order_key(to_f(z[i])) > key;
   const int need = k - block_reduce(above, Add{}, scratch);
-  uint32_t low = 0, high = (uint32_t)V - 1;   // smallest index with `need`
+  int low = 0, high = len - 1;           // smallest index that has `need`
   while (low < high) {
-    const uint32_t mid = low + (high - low) / 2;
+    const int mid = low + (high - low) / 2;
     int n = 0;
-    for (int i = threadIdx.x; i <= (int)mid; i += kThreads)
+    for (int i = threadIdx.x; i <= mid; i += NT)
       n += order_key(to_f(z[i])) == key;
     if (block_reduce(n, Add{}, scratch) >= need) high = mid;
     else low = mid + 1;
   }
   if (threadIdx.x == 0) *count = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < V; i += kThreads) {
-    const uint32_t u = order_key(to_f(z[i]));
-    if (u > key || (u == key && (uint32_t)i <= low))
-      found[atomicAdd(count, 1)] = (uint64_t)u << 32 | ~(uint32_t)i;
+  for (int i = threadIdx.x; i < len; i += NT) {
+    const float v = to_f(z[i]);
+    const uint32_t u = order_key(v);
+    if (u > key || (u == key && i <= low))
+      found[atomicAdd(count, 1)] = candidate(v, base + i);
   }
   __syncthreads();
 }
 
-// NAMED: `out` adds up the elements that no entry of `ids` names.
-template <typename T, bool NAMED>
-__device__ RowSums row_sums(const T* z, int V, float c, const int64_t* ids,
-                            int k, uint32_t* bits, double* scratch) {
-  RowSums r;
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < V; i += kThreads)
-    m = MaxNan{}(m, to_f(z[i]));
-  r.m = m = block_reduce(m, MaxNan{}, reinterpret_cast<float*>(scratch));
-  r.bad = !(fabsf(m) < INFINITY);
-  float rest = 0.f, e2 = 0.f, out = 0.f;
-  int top = 0;
-  for (int base = 0; base < V; base += kChunk) {
-    const int end = V - base < kChunk ? V - base : kChunk;
-    if constexpr (NAMED) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < kChunk / 32; i += kThreads) bits[i] = 0;
-      __syncthreads();
-      if (threadIdx.x < k) {
-        const int64_t at = ids[threadIdx.x] - base;
-        if (at >= 0 && at < end) atomicOr(&bits[at >> 5], 1u << (at & 31));
+// Lanes' values in falling order (bitonic, 21 exchanges).
+__device__ __forceinline__ float wave_sort(float v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+    for (int o = size >> 1; o > 0; o >>= 1) {
+      const float w = __shfl_xor(v, o);
+      const bool larger = ((lane & o) == 0) == ((lane & size) == 0 ||
+                                                size == 64);
+      v = larger ? fmaxf(v, w) : fminf(v, w);
+    }
+  return v;
+}
+
+// The k best of a slice into found[0..n), in no order; every thread gets n.
+// Each of NT / 64 waves has ceil(k / waves) elements that reach the smallest
+// of the waves' such maxima of threads: k elements at least reach it, and
+// about k ln(waves) do if the row is in no order. Only those are collected.
+template <typename T, int NT, int NV>
+__device__ int slice_top(const Slice<T, NT, NV>& s, const T* z, int len,
+                         int base, int k, float mine, bool has_nan,
+                         uint64_t* found, int* count, float* wave_floor,
+                         int* scratch) {
+  constexpr int W = NT / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (!has_nan) {
+    const int each = (k + W - 1) / W;
+    float bar;
+    if (each == 1) {
+      bar = wave_reduce(mine, Max{});
+    } else {
+      bar = __shfl(wave_sort(mine), each - 1);
+    }
+    if (lane == 0) wave_floor[wave] = bar;
+    if (threadIdx.x == 0) *count = 0;
+    __syncthreads();
+    bar = wave_floor[lane & (W - 1)];
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) bar = fminf(bar, __shfl_xor(bar, o));
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      if (!(s.vmax[v] >= bar)) continue;
+      const int i = Slice<T, NT, NV>::first(v);
+#pragma unroll
+      for (int j = 0; j < kVec<T>; ++j) {
+        const float x = s.at(v, j);
+        if (x >= bar && i + j < len) {
+          const int at = atomicAdd(count, 1);
+          if (at < kCandidates) found[at] = candidate(x, base + i + j);
+        }
       }
-      __syncthreads();
     }
-    for (int i = threadIdx.x; i < end; i += kThreads) {
-      const float v = to_f(z[base + i]);
-      const float y = (v - m) * c;
-      const float e = __builtin_amdgcn_exp2f(y);
-      if (v == m) ++top;
-      else rest += e;
-      e2 += e * fmaxf(y, -256.f);           // 0 for a logit of -inf
-      if constexpr (NAMED)
-        if (!(bits[i >> 5] >> (i & 31) & 1)) out += e;
-    }
+    __syncthreads();
+    const int n = *count;
+    __syncthreads();
+    if (n <= kCandidates) return n;
   }
-  const double others = block_reduce((double)rest, Add{}, scratch) +
-                        (block_reduce((double)top, Add{}, scratch) - 1.0);
-  r.s = 1.0 + others;
-  r.log_s = log1p(others);
-  r.e2 = block_reduce((double)e2, Add{}, scratch);
-  r.out = NAMED ? block_reduce((double)out, Add{}, scratch) : 0.0;
+  bisect_top<T, NT>(z, len, base, k, found, count, scratch);
+  return k;
+}
+
+// Calls put(rank, candidate) for the k best of found[0..n).
+template <int NT, typename Put>
+__device__ __forceinline__ void ranked(const uint64_t* found, int n, int k,
+                                       Put put) {
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const uint64_t mine = found[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += found[j] > mine;
+    if (rank < k) put(rank, mine);
+  }
+}
+
+// ------------------------------------------------------ sums of one slice
+struct NoBits {
+  static constexpr bool kTail = false;
+};
+// A byte for each 16-byte piece of the slice, a bit for each token of it.
+struct Bits {
+  static constexpr bool kTail = true;
+  const uint8_t* named;
+};
+
+// Adds up one slice against the maximum m (not NaN, finite). ENT: e2 too.
+// Results in the first wave's lane 0.
+template <typename T, int NT, int NV, bool ENT, typename B>
+__device__ __forceinline__ Sums slice_sums(const Slice<T, NT, NV>& s, B bits,
+                                           float m, float mine, Factor f,
+                                           float (*scratch)[6]) {
+  constexpr int W = NT / 64, E = kVec<T>;
+  float rest = 0.f, e2 = 0.f, in = 0.f, n = 0.f, n_in = 0.f;
+  auto plain = [&](int v) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const float y = (s.at(v, j) - m) * f.c;
+      const float e = __builtin_amdgcn_exp2f(y);
+      rest += e;
+      if constexpr (ENT) e2 = fmaf(e, fmaxf(y, -256.f), e2);  // 0 for -inf
+    }
+  };
+  auto careful = [&](int v, uint32_t named) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const float z = s.at(v, j);
+      const bool inside = B::kTail && (named >> j & 1);
+      if (z == m) {
+        if (inside) n_in += 1.f;
+        else n += 1.f;
+      } else {
+        const float y = (z - m) * f.c;
+        const float e = __builtin_amdgcn_exp2f(y);
+        if (inside) in += e;
+        else rest += e;
+        if constexpr (ENT) e2 = fmaf(e, fmaxf(y, -256.f), e2);
+      }
+    }
+  };
+  const bool owner = mine == m;          // holds an element equal to m
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    uint32_t named = 0;
+    if constexpr (B::kTail) named = bits.named[v * NT + threadIdx.x];
+    if (owner || named) careful(v, named);
+    else plain(v);
+  }
+  rest = wave_reduce(rest, Add{});
+  n = wave_reduce(n, Add{});
+  if constexpr (ENT) e2 = wave_reduce(e2, Add{});
+  if constexpr (B::kTail) {
+    in = wave_reduce(in, Add{});
+    n_in = wave_reduce(n_in, Add{});
+  }
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) {
+    float* p = scratch[threadIdx.x >> 6];
+    p[0] = rest; p[1] = n; p[2] = e2; p[3] = in; p[4] = n_in;
+  }
+  __syncthreads();
+  Sums r = {};
+  if (threadIdx.x < 64) {
+    const float* p = scratch[lane & (W - 1)];
+    r.rest = p[0];
+    r.n = p[1];
+    r.e2 = p[2];
+    r.in = p[3];
+    r.n_in = p[4];
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) {
+      r.rest += __shfl_xor(r.rest, o);
+      r.n += __shfl_xor(r.n, o);
+      if constexpr (ENT) r.e2 += __shfl_xor(r.e2, o);
+      if constexpr (B::kTail) {
+        r.in += __shfl_xor(r.in, o);
+        r.n_in += __shfl_xor(r.n_in, o);
+      }
+    }
+    r.m = m;
+    // exp2(y c_exact / c) of every element, to first order (2^-25 squared)
+    if constexpr (ENT) r.rest += (f.exact / (double)f.c - 1.0) * kLn2 * r.e2;
+  }
   return r;
 }
 
+// Joins the records of a row's slices; to be called by a whole wave. A slice
+// of -inf alone adds nothing.
+__device__ __forceinline__ Sums join_sums(const Sums* part, int64_t ns,
+                                          Factor f) {
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY;
+  for (int64_t i = lane; i < ns; i += 64)
+    m = MaxNan{}(m, (float)part[i].m);
+  m = wave_reduce(m, MaxNan{});
+  Sums r = {};
+  r.m = m;
+  for (int64_t i = lane; i < ns; i += 64) {
+    const Sums p = part[i];
+    if (p.m == (double)m) {
+      r.n += p.n;
+      r.rest += p.rest;
+      r.e2 += p.e2;
+      r.n_in += p.n_in;
+      r.in += p.in;
+    } else if (p.m > -INFINITY) {
+      const double y = (p.m - (double)m) * f.exact, g = exp2(y);
+      const double all = p.n + p.rest;
+      r.rest += g * all;
+      r.e2 += g == 0.0 ? 0.0 : g * (p.e2 + y * all);
+      r.in += g * (p.n_in + p.in);
+    }
+  }
+  for (int o = 32; o > 0; o >>= 1) {
+    r.n += __shfl_xor(r.n, o);
+    r.rest += __shfl_xor(r.rest, o);
+    r.e2 += __shfl_xor(r.e2, o);
+    r.n_in += __shfl_xor(r.n_in, o);
+    r.in += __shfl_xor(r.in, o);
+  }
+  return r;
+}
+
+// --------------------------------------------------- log probabilities, forward
+struct LogprobArgs {
+  const int64_t* tokens;
+  int64_t zs, ignore, rows;
+  int V, k, per_slice;       // tokens of a slice
+  int64_t slices;
+  Factor f;
+  double inv_t;
+  float *logprob, *entropy, *top_lp;
+  int64_t* top_ids;
+  RowStats* stats;
+  Sums* part;                // [rows][slices], of more than one slice
+  uint64_t* lists;           // [rows][slices][k], best first, 0: no such one
+};
+
+// One thread: everything of a row but its top; returns log s (NaN: bad).
 template <typename T>
-__global__ __launch_bounds__(kThreads) void logprobs_fwd_kernel(
-    const T* __restrict__ logits, int64_t zs,
-    const int64_t* __restrict__ tokens, int64_t ignore, int64_t rows, int V,
-    int k, float c, double inv_t, float* __restrict__ logprob,
-    float* __restrict__ entropy, float* __restrict__ top_lp,
-    int64_t* __restrict__ top_ids, RowStats* __restrict__ stats) {
-  __shared__ double scratch[kThreads / 64];
-  __shared__ uint64_t found[kMaxTop];
-  __shared__ int count;
-  const int tid = threadIdx.x;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T* z = logits + row * zs;
-    const int64_t token = tokens ? tokens[row] : 0;
-    if (tokens && token == ignore) {
-      if (tid == 0) {
-        logprob[row] = 0.f;
-        entropy[row] = 0.f;
-        if (stats) stats[row] = {0.f, 0.f, 0.f, 0.f};
-      }
-      for (int i = tid; i < k; i += kThreads) {
-        top_lp[row * k + i] = -INFINITY;
-        top_ids[row * k + i] = -1;
-      }
-      continue;
-    }
-    const RowSums r = row_sums<T, false>(z, V, c, nullptr, 0, nullptr,
-                                         scratch);
-    if (tid == 0) {
-      const double h = r.bad ? NAN : r.log_s - kLn2 * r.e2 / r.s;
-      entropy[row] = (float)h;
-      if (tokens) {
-        const bool ok = token >= 0 && token < V && !r.bad;
-        logprob[row] =
-            ok ? (float)(((double)to_f(z[token]) - (double)r.m) * inv_t -
-                         r.log_s)
-               : NAN;
-      }
-      if (stats)
-        stats[row] = {r.m, r.bad ? NAN : (float)(1.0 / r.s),
-                      (float)(h - r.log_s), 0.f};
-    }
-    if (k) {
-      row_top(z, V, k, found, &count, reinterpret_cast<int*>(scratch));
-      if (tid < k) {
-        const uint64_t mine = found[tid];
-        int rank = 0;
-        for (int i = 0; i < k; ++i) rank += found[i] > mine;
-        const uint32_t id = ~(uint32_t)mine;
-        top_ids[row * k + rank] = id;
-        top_lp[row * k + rank] =
-            r.bad ? NAN
-                  : (float)(((double)to_f(z[id]) - (double)r.m) * inv_t -
-                            r.log_s);
-      }
-      __syncthreads();
-    }
+__device__ __forceinline__ double finish_logprob(const LogprobArgs& a,
+                                                 int64_t row, const T* z,
+                                                 const Sums& s) {
+  const float m = (float)s.m;
+  const bool bad = no_distribution(m);
+  const double others = s.rest + (s.n - 1.0), sum = 1.0 + others;
+  const double log_s = bad ? NAN : log1p(others);
+  const double h = log_s - kLn2 * s.e2 / sum;
+  a.entropy[row] = (float)h;
+  if (a.tokens) {
+    const int64_t token = a.tokens[row];
+    const bool known = token >= 0 && token < a.V;
+    a.logprob[row] =
+        known ? (float)(((double)to_f(z[token]) - s.m) * a.inv_t - log_s)
+              : NAN;
+  }
+  if (a.stats)
+    a.stats[row] = {m, bad ? NAN : (float)(1.0 / sum), (float)(h - log_s),
+                    0.f};
+  return log_s;
+}
+
+__device__ __forceinline__ void skip_logprob(const LogprobArgs& a,
+                                             int64_t row) {
+  if (threadIdx.x == 0) {
+    a.logprob[row] = 0.f;
+    a.entropy[row] = 0.f;
+    if (a.stats) a.stats[row] = {0.f, 0.f, 0.f, 0.f};
+  }
+  for (int i = threadIdx.x; i < a.k; i += blockDim.x) {
+    a.top_lp[row * a.k + i] = -INFINITY;
+    a.top_ids[row * a.k + i] = -1;
   }
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void logprobs_bwd_kernel(
-    const T* __restrict__ logits, int64_t zs,
-    const int64_t* __restrict__ tokens, const int64_t* __restrict__ top_ids,
-    const RowStats* __restrict__ stats, const float* __restrict__ d_logprob,
-    const float* __restrict__ d_entropy, const float* __restrict__ d_top,
-    T* __restrict__ dz, int64_t rows, int V, int k, float c, float inv_t) {
-  __shared__ float scratch[kThreads / 64];
-  const int tid = threadIdx.x;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T* z = logits + row * zs;
-    T* out = dz + row * V;
-    const RowStats s = stats[row];
-    if (s.inv_s == 0.f) {
-      for (int i = tid; i < V; i += kThreads) out[i] = static_cast<T>(0.f);
+__device__ __forceinline__ void put_top(const LogprobArgs& a, int64_t row,
+                                        const T* z, int rank, int id, double m,
+                                        double log_s) {
+  a.top_ids[row * a.k + rank] = id;
+  a.top_lp[row * a.k + rank] =
+      (float)(((double)to_f(z[id]) - m) * a.inv_t - log_s);
+}
+
+template <typename T, int NT, int NV, bool TOP>
+__global__ __launch_bounds__(NT) void logprobs_slice_kernel(
+    const T* __restrict__ logits, const LogprobArgs a) {
+  __shared__ float wave_max[NT / 64], wave_floor[NT / 64];
+  __shared__ float sums[NT / 64][6];
+  __shared__ int scratch[NT / 64];
+  __shared__ uint64_t found[TOP ? kCandidates : 1];
+  __shared__ double log_sum;
+  __shared__ int count;
+  const int64_t work = a.rows * a.slices;
+  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
+    const int64_t row = a.slices == 1 ? w : w / a.slices;
+    const int base = (int)(w - row * a.slices) * a.per_slice;
+    if (a.tokens && a.tokens[row] == a.ignore) {
+      if (base == 0) skip_logprob(a, row);
       continue;
     }
-    const int64_t token = d_logprob ? tokens[row] : -1;
-    const float up = d_logprob ? d_logprob[row] : 0.f;
-    const float dh = d_entropy ? d_entropy[row] : 0.f;
-    float a = d_top && tid < k ? d_top[row * k + tid] : 0.f;
-    a = block_reduce(a, Add{}, scratch) + up;
-    // a token outside of the vocabulary has no gradient that is a number
-    if (d_logprob && (token < 0 || token >= V)) a = NAN;
-    auto base = [&](float v) {
-      const float d = v - s.m;
-      const float p = __builtin_amdgcn_exp2f(d * c) * s.inv_s;
-      float f = a;
-      if (d_entropy) f += dh * (fmaxf(d * inv_t, -1e30f) + s.a);
-      return -p * f;
-    };
-    for (int i = tid; i < V; i += kThreads)
-      out[i] = static_cast<T>(base(to_f(z[i])) * inv_t);
-    __syncthreads();
-    // the named tokens once more, with what is theirs: thread k has the token
-    if (tid <= k) {
-      const int64_t id = tid == k ? token
-                         : d_top  ? top_ids[row * k + tid]
-                                  : -1;
-      if (id >= 0 && id < V) {
-        float g = id == token ? up : 0.f;
-        if (d_top)
-          for (int i = 0; i < k; ++i)
-            if (top_ids[row * k + i] == id) g += d_top[row * k + i];
-        out[id] = static_cast<T>((base(to_f(z[id])) + g) * inv_t);
+    const T* z = logits + row * a.zs;
+    const int len = min(a.per_slice, a.V - base);
+    Slice<T, NT, NV> s;
+    s.load(z + base, len);
+    const float mine = s.max();
+    const float m = block_max<NT>(mine, wave_max);
+    Sums r = {};
+    if (!no_distribution(m))
+      r = slice_sums<T, NT, NV, true>(s, NoBits{}, m, mine, a.f, sums);
+    r.m = m;
+    if (threadIdx.x == 0) {
+      if (a.slices == 1) log_sum = finish_logprob(a, row, z, r);
+      else a.part[w] = r;
+    }
+    if constexpr (TOP) {
+      const int k = min(a.k, len);
+      const int n = slice_top(s, z + base, len, base, k, mine, m != m, found,
+                              &count, wave_floor, scratch);
+      if (a.slices == 1) {
+        const double log_s = log_sum;    // slice_top has synchronised
+        ranked<NT>(found, n, k, [&](int rank, uint64_t c) {
+          put_top(a, row, z, rank, id_of(c), (double)m, log_s);
+        });
+      } else {
+        uint64_t* list = a.lists + w * a.k;
+        ranked<NT>(found, n, k, [&](int rank, uint64_t c) { list[rank] = c; });
+        for (int i = k + threadIdx.x; i < a.k; i += NT) list[i] = 0;
       }
+    }
+    __syncthreads();                     // before the arrays are used again
+  }
+}
+
+// Rows of more than one slice: a block of 256 joins the records of one row.
+template <typename T>
+__global__ __launch_bounds__(256) void logprobs_join_kernel(
+    const T* __restrict__ logits, const LogprobArgs a) {
+  __shared__ double shared[2];
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    if (a.tokens && a.tokens[row] == a.ignore) continue;
+    const T* z = logits + row * a.zs;
+    if (threadIdx.x < 64) {
+      const Sums s = join_sums(a.part + row * a.slices, a.slices, a.f);
+      if (threadIdx.x == 0) {
+        shared[0] = finish_logprob(a, row, z, s);
+        shared[1] = s.m;
+      }
+    }
+    __syncthreads();
+    const double log_s = shared[0], m = shared[1];
+    // the place of a candidate: its place in its own list, and how many of
+    // each other list are better
+    const uint64_t* lists = a.lists + row * a.slices * a.k;
+    for (int64_t i = threadIdx.x; i < a.slices * a.k; i += 256) {
+      const uint64_t mine = lists[i];
+      if (mine == 0) continue;
+      const int64_t own = i / a.k;
+      int64_t rank = i - own * a.k;
+      for (int64_t l = 0; l < a.slices && rank < a.k; ++l) {
+        if (l == own) continue;
+        const uint64_t* list = lists + l * a.k;
+        int lo = 0, hi = a.k;            // entries that are better
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (list[mid] > mine) lo = mid + 1;
+          else hi = mid;
+        }
+        rank += lo;
+      }
+      if (rank < a.k) put_top(a, row, z, (int)rank, id_of(mine), m, log_s);
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------ distillation, forward
+struct DistillArgs {
+  const int64_t* ids;
+  const float* teacher;
+  int64_t zs, rows;
+  int V, k, per_slice;
+  int64_t slices;
+  Factor f;
+  double t;
+  float *loss, *q_out;
+  RowStats* stats;
+  Sums* part;
+};
+
+// Whole block, of 256 threads or more; s: in every thread.
+template <typename T, bool TAIL>
+__device__ void finish_distill(const DistillArgs& a, int64_t row, const T* z,
+                               const Sums& s, int64_t id, double* scratch,
+                               double* shares, int64_t* named) {
+  const int tid = threadIdx.x, k = a.k;
+  const bool present = id >= 0;
+  const float lp = present ? a.teacher[row * k + tid] : -INFINITY;
+  double q, rest = 0.0;
+  if constexpr (TAIL) {
+    q = exp((double)lp);
+    const double left = 1.0 - block_reduce(q, Add{}, scratch);
+    rest = left <= 0.0 ? 0.0 : left;
+  } else {
+    const float top = block_reduce(lp, MaxNan{},
+                                   reinterpret_cast<float*>(scratch));
+    q = top == -INFINITY ? 0.0 : exp((double)lp - (double)top);
+    const double sum = block_reduce(q, Add{}, scratch);
+    q = sum == 0.0 ? 0.0 : q / sum;
+  }
+  const float m = (float)s.m;
+  const double outside = s.n + s.rest;
+  const double others = (s.rest + s.in) + ((s.n + s.n_in) - 1.0);
+  const double sum = 1.0 + others, log_s = log1p(others);
+  double term = 0.0;
+  if (id >= a.V) term = NAN;                 // no such token
+  else if (present && q != 0.0)
+    term = q * (log(q) - (((double)to_f(z[id]) - s.m) / a.t - log_s));
+  double total = block_reduce(term, Add{}, scratch);
+  double share = block_reduce(q, Add{}, scratch), shift = 0.0;
+  if (TAIL && rest != 0.0 && outside > 0.0) {
+    share += rest;
+    total += rest * (log(rest) - (log(outside) - log_s));
+    shift = rest * sum / outside;
+  }
+  if (no_distribution(m)) total = NAN;
+  if (tid == 0) a.loss[row] = (float)(total * a.t * a.t);
+  if (a.stats) {
+    if (tid == 0)
+      a.stats[row] = {m, total != total ? NAN : (float)(1.0 / sum),
+                      (float)share, (float)(share - shift)};
+    // an id that is named more than once: each entry gets the sum
+    if (tid < k) {
+      shares[tid] = q;
+      named[tid] = id;
+    }
+    __syncthreads();
+    if (tid < k) {
+      double all = 0.0;
+      for (int i = 0; i < k; ++i) all += named[i] == id ? shares[i] : 0.0;
+      a.q_out[row * k + tid] = (float)all;
+    }
+  }
+}
+
+__device__ __forceinline__ void skip_distill(const DistillArgs& a,
+                                             int64_t row) {
+  if (threadIdx.x == 0) {
+    a.loss[row] = 0.f;
+    if (a.stats) a.stats[row] = {0.f, 0.f, 0.f, 0.f};
+  }
+  if (a.stats && threadIdx.x < a.k) a.q_out[row * a.k + threadIdx.x] = 0.f;
+}
+
+template <typename T, int NT, int NV, bool TAIL>
+__global__ __launch_bounds__(NT) void distill_slice_kernel(
+    const T* __restrict__ logits, const DistillArgs a) {
+  __shared__ float wave_max[NT / 64];
+  __shared__ float sums[NT / 64][6];
+  __shared__ double scratch[NT / 64], shares[kMaxTop];
+  __shared__ int64_t named[kMaxTop];
+  __shared__ Sums whole;
+  __shared__ uint32_t bits[TAIL ? NT * NV / 4 : 1];
+  const int64_t work = a.rows * a.slices;
+  const int tid = threadIdx.x;
+  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
+    const int64_t row = a.slices == 1 ? w : w / a.slices;
+    const int base = (int)(w - row * a.slices) * a.per_slice;
+    const int64_t id = tid < a.k ? a.ids[row * a.k + tid] : -1;
+    if constexpr (TAIL)
+      for (int i = tid; i < NT * NV / 4; i += NT) bits[i] = 0;
+    if (!__syncthreads_or(id >= 0)) {
+      if (base == 0) skip_distill(a, row);
+      continue;
+    }
+    const T* z = logits + row * a.zs;
+    const int len = min(a.per_slice, a.V - base);
+    Slice<T, NT, NV> s;
+    s.load(z + base, len);
+    if constexpr (TAIL) {
+      const int64_t at = id - base;
+      if (at >= 0 && at < len) {
+        constexpr int E = kVec<T>;
+        const int piece = (int)at / E, bit = (int)at % E;
+        atomicOr(&bits[piece / 4], 1u << (piece % 4 * 8 + bit));
+      }
+    }
+    const float mine = s.max();
+    const float m = block_max<NT>(mine, wave_max);   // synchronises
+    Sums r = {};
+    if (!no_distribution(m)) {
+      if constexpr (TAIL)
+        r = slice_sums<T, NT, NV, false>(
+            s, Bits{reinterpret_cast<const uint8_t*>(bits)}, m, mine, a.f,
+            sums);
+      else
+        r = slice_sums<T, NT, NV, false>(s, NoBits{}, m, mine, a.f, sums);
+    }
+    r.m = m;
+    if (a.slices == 1) {
+      if (tid == 0) whole = r;
+      __syncthreads();
+      finish_distill<T, TAIL>(a, row, z, whole, id, scratch, shares, named);
+    } else if (tid == 0) {
+      a.part[w] = r;
     }
     __syncthreads();
   }
 }
 
 template <typename T, bool TAIL>
-__global__ __launch_bounds__(kThreads) void distill_fwd_kernel(
-    const T* __restrict__ logits, int64_t zs,
-    const int64_t* __restrict__ ids, const float* __restrict__ teacher,
-    int64_t rows, int V, int k, float c, double t, float* __restrict__ loss,
-    float* __restrict__ q_out, RowStats* __restrict__ stats) {
-  __shared__ double scratch[kThreads / 64];
-  __shared__ uint32_t bits[TAIL ? kChunk / 32 : 1];
+__global__ __launch_bounds__(256) void distill_join_kernel(
+    const T* __restrict__ logits, const DistillArgs a) {
+  __shared__ double scratch[4], shares[kMaxTop];
+  __shared__ int64_t named[kMaxTop];
+  __shared__ Sums whole;
   const int tid = threadIdx.x;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T* z = logits + row * zs;
-    const int64_t id = tid < k ? ids[row * k + tid] : -1;
-    const bool present = id >= 0;
-    const bool live = block_reduce((int)present, Add{},
-                                   reinterpret_cast<int*>(scratch)) > 0;
-    if (!live) {
-      if (tid == 0) loss[row] = 0.f;
-      if (stats) {
-        if (tid == 0) stats[row] = {0.f, 0.f, 0.f, 0.f};
-        if (tid < k) q_out[row * k + tid] = 0.f;
-      }
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int64_t id = tid < a.k ? a.ids[row * a.k + tid] : -1;
+    if (!__syncthreads_or(id >= 0)) continue;
+    if (tid < 64) {
+      const Sums s = join_sums(a.part + row * a.slices, a.slices, a.f);
+      if (tid == 0) whole = s;
+    }
+    __syncthreads();
+    finish_distill<T, TAIL>(a, row, logits + row * a.zs, whole, id, scratch,
+                            shares, named);
+    __syncthreads();
+  }
+}
+
+// ----------------------------------------------------------------- backward
+// A block of 256 takes a piece of 256 * kPieces vectors of one row.
+constexpr int kBwdThreads = 256;
+constexpr int kPieces = 4;
+template <typename T>
+constexpr int kBwdTokens = kBwdThreads * kPieces * kVec<T>;
+
+template <typename T, typename F>
+__device__ __forceinline__ void map_piece(const T* z, T* out, int len, F f) {
+  constexpr int E = kVec<T>;
+  u32x4 v[kPieces];
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p) {
+    const int i = (p * kBwdThreads + (int)threadIdx.x) * E;
+    if (i + E <= len) v[p] = load16(z + i);
+  }
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p) {
+    const int i = (p * kBwdThreads + (int)threadIdx.x) * E;
+    if (i + E <= len) {
+      float r[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) r[j] = f(elem<T>(v[p], j));
+      store16(out + i, pack<T>(r));
+    } else {
+      for (int j = i; j < len; ++j) out[j] = static_cast<T>(f(to_f(z[j])));
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void zero_piece(T* out, int len) {
+  constexpr int E = kVec<T>;
+#pragma unroll
+  for (int p = 0; p < kPieces; ++p) {
+    const int i = (p * kBwdThreads + (int)threadIdx.x) * E;
+    if (i + E <= len) store16(out + i, u32x4{0, 0, 0, 0});
+    else
+      for (int j = i; j < len; ++j) out[j] = static_cast<T>(0.f);
+  }
+}
+
+template <typename T, bool ENT>
+__global__ __launch_bounds__(kBwdThreads) void logprobs_bwd_kernel(
+    const T* __restrict__ logits, int64_t zs,
+    const int64_t* __restrict__ tokens, const int64_t* __restrict__ top_ids,
+    const RowStats* __restrict__ stats, const float* __restrict__ d_logprob,
+    const float* __restrict__ d_entropy, const float* __restrict__ d_top,
+    T* __restrict__ dz, int64_t rows, int V, int64_t pieces, int k, float c,
+    float inv_t) {
+  __shared__ int token_in_top;
+  const int tid = threadIdx.x;
+  for (int64_t w = blockIdx.x; w < rows * pieces; w += gridDim.x) {
+    const int64_t row = w / pieces;
+    const int base = (int)(w - row * pieces) * kBwdTokens<T>;
+    const int len = min(kBwdTokens<T>, V - base);
+    const T* z = logits + row * zs + base;
+    T* out = dz + row * V + base;
+    const RowStats s = stats[row];
+    if (s.inv_s == 0.f) {
+      zero_piece(out, len);
       continue;
     }
-    const float lp = present ? teacher[row * k + tid] : -INFINITY;
-    double q, rest = 0.0;
-    if constexpr (TAIL) {
-      q = exp((double)lp);
-      const double left = 1.0 - block_reduce(q, Add{}, scratch);
-      rest = left <= 0.0 ? 0.0 : left;
-    } else {
-      const float top = block_reduce(lp, MaxNan{},
-                                     reinterpret_cast<float*>(scratch));
-      q = top == -INFINITY ? 0.0 : exp((double)lp - (double)top);
-      const double sum = block_reduce(q, Add{}, scratch);
-      q = sum == 0.0 ? 0.0 : q / sum;
+    const int64_t token = d_logprob ? tokens[row] : -1;
+    const float up = d_logprob ? d_logprob[row] : 0.f;
+    const float dh = ENT ? d_entropy[row] : 0.f;
+    float a = 0.f;
+    if (d_top) {
+      for (int i = tid & 63; i < k; i += 64) a += d_top[row * k + i];
+      a = wave_reduce(a, Add{});
     }
-    const RowSums r = row_sums<T, TAIL>(z, V, c, ids + row * k, k, bits,
-                                        scratch);
-    double term = 0.0;
-    if (id >= V) term = NAN;                 // no such token
-    else if (present && q != 0.0)
-      term = q * (log(q) -
-                  (((double)to_f(z[id]) - (double)r.m) / t - r.log_s));
-    double total = block_reduce(term, Add{}, scratch);
-    double share = block_reduce(q, Add{}, scratch), shift = 0.0;
-    if (TAIL && rest != 0.0 && r.out > 0.0) {
-      share += rest;
-      total += rest * (log(rest) - (log(r.out) - r.log_s));
-      shift = rest * r.s / r.out;
+    a += up;
+    // a token outside of the vocabulary has no gradient that is a number
+    if (d_logprob && (token < 0 || token >= V)) a = NAN;
+    const float scale = -s.inv_s * inv_t;
+    auto spread = [&](float v) {
+      const float y = (v - s.m) * c;
+      const float e = __builtin_amdgcn_exp2f(y) * scale;
+      if constexpr (ENT)
+        return e * fmaf(dh, fmaf(fmaxf(y, -1e30f), (float)kLn2, s.a), a);
+      return e * a;
+    };
+    map_piece(z, out, len, spread);
+    if (!d_logprob && !d_top) continue;
+    // the named tokens of this piece again, with what is theirs; the token
+    // itself where it is not one of the top
+    if (tid == 0) token_in_top = 0;
+    __syncthreads();
+    if (d_top && tid < k) {
+      const int64_t id = top_ids[row * k + tid];
+      float g = d_top[row * k + tid];
+      if (id == token) {
+        g += up;
+        token_in_top = 1;
+      }
+      if (id >= base && id - base < len) {
+        const int i = (int)(id - base);
+        out[i] = static_cast<T>(fmaf(g, inv_t, spread(to_f(z[i]))));
+      }
     }
-    if (r.bad) total = NAN;
-    if (tid == 0) loss[row] = (float)(total * t * t);
-    if (stats) {
-      if (tid == 0)
-        stats[row] = {r.m, total != total ? NAN : (float)(1.0 / r.s),
-                      (float)share, (float)(share - shift)};
-      if (tid < k) q_out[row * k + tid] = (float)q;
+    __syncthreads();
+    if (tid == 0 && !token_in_top && token >= base && token - base < len) {
+      const int i = (int)(token - base);
+      out[i] = static_cast<T>(fmaf(up, inv_t, spread(to_f(z[i]))));
     }
     __syncthreads();
   }
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void distill_bwd_kernel(
+__global__ __launch_bounds__(kBwdThreads) void distill_bwd_kernel(
     const T* __restrict__ logits, int64_t zs,
     const int64_t* __restrict__ ids, const float* __restrict__ q,
     const RowStats* __restrict__ stats, const float* __restrict__ d_loss,
-    T* __restrict__ dz, int64_t rows, int V, int k, float c, float t) {
+    T* __restrict__ dz, int64_t rows, int V, int64_t pieces, int k, float c,
+    float t) {
   const int tid = threadIdx.x;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T* z = logits + row * zs;
-    T* out = dz + row * V;
+  for (int64_t w = blockIdx.x; w < rows * pieces; w += gridDim.x) {
+    const int64_t row = w / pieces;
+    const int base = (int)(w - row * pieces) * kBwdTokens<T>;
+    const int len = min(kBwdTokens<T>, V - base);
+    const T* z = logits + row * zs + base;
+    T* out = dz + row * V + base;
     const RowStats s = stats[row];
     if (s.inv_s == 0.f) {
-      for (int i = tid; i < V; i += kThreads) out[i] = static_cast<T>(0.f);
+      zero_piece(out, len);
       continue;
     }
-    const float g = d_loss[row] * t;
-    for (int i = tid; i < V; i += kThreads) {
-      const float p = __builtin_amdgcn_exp2f((to_f(z[i]) - s.m) * c) * s.inv_s;
-      out[i] = static_cast<T>(p * s.b * g);
-    }
+    const float g = d_loss[row] * t, outside = s.inv_s * s.b * g;
+    map_piece(z, out, len, [&](float v) {
+      return __builtin_amdgcn_exp2f((v - s.m) * c) * outside;
+    });
     __syncthreads();
     if (tid < k) {
       const int64_t id = ids[row * k + tid];
-      if (id >= 0 && id < V) {
-        float taught = 0.f;
-        for (int i = 0; i < k; ++i)
-          if (ids[row * k + i] == id) taught += q[row * k + i];
+      if (id >= base && id - base < len) {
+        const int i = (int)(id - base);
         const float p =
-            __builtin_amdgcn_exp2f((to_f(z[id]) - s.m) * c) * s.inv_s;
-        out[id] = static_cast<T>((p * s.a - taught) * g);
+            __builtin_amdgcn_exp2f((to_f(z[i]) - s.m) * c) * s.inv_s;
+        out[i] = static_cast<T>((p * s.a - q[row * k + tid]) * g);
       }
     }
-    __syncthreads();
   }
 }
 
-int grid_for(int64_t rows) {
-  return (int)(rows < kMaxBlocks ? rows : kMaxBlocks);
+// ------------------------------------------------------------------ launches
+int grid_for(int64_t work) {
+  return (int)(work < kMaxBlocks ? work : kMaxBlocks);
 }
 
 // log2(e) / T: exp(t) is exp2 of the distance times this
-float exp2_factor(double t) { return (float)(1.4426950408889634074 / t); }
+Factor exp2_factor(double t) {
+  const double exact = 1.4426950408889634074 / t;
+  return {(float)exact, exact};
+}
+
+// Threads and 16-byte vectors of a slice: the smallest block that holds the
+// row, up to 8192 vectors; longer rows in equal slices.
+struct Cut {
+  int threads, vectors, per_slice;
+  int64_t slices;
+};
+
+Cut cut_row(int V, int per_vector) {
+  const int64_t vecs = (V + per_vector - 1) / per_vector;
+  const int64_t few = (vecs + 8191) / 8192;
+  const int64_t each = (vecs + few - 1) / few;
+  const int64_t slices = (vecs + each - 1) / each;     // none of them empty
+  const int threads = each <= 1024 ? 256 : 1024;
+  const int vectors = each <= 256 ? 1 : each <= 1024 || each <= 4096 ? 4 : 8;
+  return {threads, vectors, (int)(each * per_vector), slices};
+}
+
+template <typename F>
+void with_cut(const Cut& c, F f) {
+  if (c.threads == 256 && c.vectors == 1) f(Int<256>{}, Int<1>{});
+  else if (c.threads == 256) f(Int<256>{}, Int<4>{});
+  else if (c.vectors == 4) f(Int<1024>{}, Int<4>{});
+  else f(Int<1024>{}, Int<8>{});
+}
+
+template <typename F>
+void with_type(int type, F f) {
+  if (type == kF32) f(float{});
+  else if (type == kBF16) f(bf16{});
+  else f(f16{});
+}
+
+int per_vector(int type) { return type == kF32 ? 4 : 8; }
 
 }  // namespace
 
-#define BY_TYPE(type, CALL)                                                   \
-  if ((type) == kF32) CALL(float);                                            \
-  else if ((type) == kBF16) CALL(bf16);                                       \
-  else CALL(f16)
+// Slices of a row, and bytes of the record that each leaves where there is
+// more than one.
+int64_t dear_logit_slices(int type, int V) {
+  return cut_row(V, per_vector(type)).slices;
+}
+int64_t dear_slice_bytes() { return sizeof(Sums); }
 
 int dear_logprobs_fwd(hipStream_t st, int type, const void* logits, int64_t zs,
                       const int64_t* tokens, int64_t ignore, int64_t rows,
                       int V, int k, double t, float* logprob, float* entropy,
-                      float* top_lp, int64_t* top_ids, void* stats) {
-#define CALL(T)                                                               \
-  hipLaunchKernelGGL((logprobs_fwd_kernel<T>), dim3(grid_for(rows)), dim3(kThreads), 0, st,                 \
-      (const T*)logits, zs, tokens, ignore, rows, V, k, exp2_factor(t),       \
-      1.0 / t, logprob, entropy, top_lp, top_ids, (RowStats*)stats)
-  BY_TYPE(type, CALL);
-#undef CALL
+                      float* top_lp, int64_t* top_ids, void* stats, void* part,
+                      void* lists) {
+  const Cut cut = cut_row(V, per_vector(type));
+  const LogprobArgs a = {tokens, zs, ignore, rows, V, k, cut.per_slice,
+                         cut.slices, exp2_factor(t), 1.0 / t, logprob, entropy,
+                         top_lp, top_ids, (RowStats*)stats, (Sums*)part,
+                         (uint64_t*)lists};
+  with_type(type, [&](auto zero) {
+    using T = decltype(zero);
+    with_cut(cut, [&](auto nt, auto nv) {
+      constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
+      const dim3 grid(grid_for(rows * cut.slices)), block(NT);
+      if (k)
+        hipLaunchKernelGGL((logprobs_slice_kernel<T, NT, NV, true>), grid,
+                           block, 0, st, (const T*)logits, a);
+      else
+        hipLaunchKernelGGL((logprobs_slice_kernel<T, NT, NV, false>), grid,
+                           block, 0, st, (const T*)logits, a);
+    });
+    if (cut.slices > 1)
+      hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3(grid_for(rows)),
+                         dim3(256), 0, st, (const T*)logits, a);
+  });
   return (int)hipGetLastError();
 }
 
@@ -372,33 +902,57 @@ int dear_logprobs_bwd(hipStream_t st, int type, const void* logits, int64_t zs,
                       const void* stats, const float* d_logprob,
                       const float* d_entropy, const float* d_top, void* dz,
                       int64_t rows, int V, int k, double t) {
-#define CALL(T)                                                               \
-  hipLaunchKernelGGL((logprobs_bwd_kernel<T>), dim3(grid_for(rows)), dim3(kThreads), 0, st,                 \
-      (const T*)logits, zs, tokens, top_ids, (const RowStats*)stats,          \
-      d_logprob, d_entropy, d_top, (T*)dz, rows, V, k, exp2_factor(t),        \
-      (float)(1.0 / t))
-  BY_TYPE(type, CALL);
-#undef CALL
+  with_type(type, [&](auto zero) {
+    using T = decltype(zero);
+    const int64_t pieces = ((int64_t)V + kBwdTokens<T> - 1) / kBwdTokens<T>;
+    const dim3 grid(grid_for(rows * pieces)), block(kBwdThreads);
+    const float c = exp2_factor(t).c, inv_t = (float)(1.0 / t);
+    const RowStats* s = (const RowStats*)stats;
+    if (d_entropy)
+      hipLaunchKernelGGL((logprobs_bwd_kernel<T, true>), grid, block, 0, st,
+                         (const T*)logits, zs, tokens, top_ids, s, d_logprob,
+                         d_entropy, d_top, (T*)dz, rows, V, pieces, k, c,
+                         inv_t);
+    else
+      hipLaunchKernelGGL((logprobs_bwd_kernel<T, false>), grid, block, 0, st,
+                         (const T*)logits, zs, tokens, top_ids, s, d_logprob,
+                         d_entropy, d_top, (T*)dz, rows, V, pieces, k, c,
+                         inv_t);
+  });
   return (int)hipGetLastError();
 }
 
 int dear_distill_fwd(hipStream_t st, int type, bool tail, const void* logits,
                      int64_t zs, const int64_t* ids, const float* teacher,
                      int64_t rows, int V, int k, double t, float* loss,
-                     float* q, void* stats) {
-#define CALL(T)                                                               \
-  if (tail)                                                                   \
-    hipLaunchKernelGGL((distill_fwd_kernel<T, true>), dim3(grid_for(rows)), dim3(kThreads), 0, st,          \
-        (const T*)logits, zs, ids, teacher, rows, V, k, exp2_factor(t), t,    \
-        loss, q, (RowStats*)stats);                                           \
-  else                                                                        \
-    hipLaunchKernelGGL((distill_fwd_kernel<T, false>), dim3(grid_for(rows)), dim3(kThreads), 0, st,         \
-        (const T*)logits, zs, ids, teacher, rows, V, k, exp2_factor(t), t,    \
-        loss, q, (RowStats*)stats)
-  if (type == kF32) { CALL(float); }
-  else if (type == kBF16) { CALL(bf16); }
-  else { CALL(f16); }
-#undef CALL
+                     float* q, void* stats, void* part) {
+  const Cut cut = cut_row(V, per_vector(type));
+  const DistillArgs a = {ids, teacher, zs, rows, V, k, cut.per_slice,
+                         cut.slices, exp2_factor(t), t, loss, q,
+                         (RowStats*)stats, (Sums*)part};
+  with_type(type, [&](auto zero) {
+    using T = decltype(zero);
+    with_cut(cut, [&](auto nt, auto nv) {
+      constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
+      const dim3 grid(grid_for(rows * cut.slices)), block(NT);
+      if (tail)
+        hipLaunchKernelGGL((distill_slice_kernel<T, NT, NV, true>), grid,
+                           block, 0, st, (const T*)logits, a);
+      else
+        hipLaunchKernelGGL((distill_slice_kernel<T, NT, NV, false>), grid,
+                           block, 0, st, (const T*)logits, a);
+    });
+    if (cut.slices > 1) {
+      if (tail)
+        hipLaunchKernelGGL((distill_join_kernel<T, true>),
+                           dim3(grid_for(rows)), dim3(256), 0, st,
+                           (const T*)logits, a);
+      else
+        hipLaunchKernelGGL((distill_join_kernel<T, false>),
+                           dim3(grid_for(rows)), dim3(256), 0, st,
+                           (const T*)logits, a);
+    }
+  });
   return (int)hipGetLastError();
 }
 
@@ -406,11 +960,13 @@ int dear_distill_bwd(hipStream_t st, int type, const void* logits, int64_t zs,
                      const int64_t* ids, const float* q, const void* stats,
                      const float* d_loss, void* dz, int64_t rows, int V, int k,
                      double t) {
-#define CALL(T)                                                               \
-  hipLaunchKernelGGL((distill_bwd_kernel<T>), dim3(grid_for(rows)), dim3(kThreads), 0, st,                  \
-      (const T*)logits, zs, ids, q, (const RowStats*)stats, d_loss, (T*)dz,   \
-      rows, V, k, exp2_factor(t), (float)t)
-  BY_TYPE(type, CALL);
-#undef CALL
+  with_type(type, [&](auto zero) {
+    using T = decltype(zero);
+    const int64_t pieces = ((int64_t)V + kBwdTokens<T> - 1) / kBwdTokens<T>;
+    hipLaunchKernelGGL((distill_bwd_kernel<T>), dim3(grid_for(rows * pieces)),
+                       dim3(kBwdThreads), 0, st, (const T*)logits, zs, ids, q,
+                       (const RowStats*)stats, d_loss, (T*)dz, rows, V, pieces,
+                       k, exp2_factor(t).c, (float)t);
+  });
   return (int)hipGetLastError();
 }
