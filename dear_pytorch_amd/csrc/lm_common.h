@@ -119,6 +119,49 @@ struct MaxNan {
   }
 };
 
+// The value of a lane and of the one O lanes away (lane ^ O), in either order,
+// without a trip through LDS: quad_perm, row_half_mirror and row_ror of the
+// data-parallel primitives within rows of 16, swaps of rows beyond.
+struct Pair {
+  float x, y;
+};
+template <int Ctrl>
+__device__ __forceinline__ float dpp(float v) {
+  const int i = __float_as_int(v);
+  return __int_as_float(
+      __builtin_amdgcn_update_dpp(i, i, Ctrl, 0xf, 0xf, false));
+}
+template <int O>
+__device__ __forceinline__ Pair lanes(float v) {
+  if constexpr (O == 1) return {v, dpp<0xb1>(v)};            // quad [1,0,3,2]
+  else if constexpr (O == 2) return {v, dpp<0x4e>(v)};       // quad [2,3,0,1]
+  else if constexpr (O == 4) return {v, dpp<0x141>(dpp<0x1b>(v))};  // 3, then 7
+  else if constexpr (O == 8) return {v, dpp<0x128>(v)};      // rotate by 8
+  else {
+    const uint32_t u = __float_as_uint(v);
+    const auto r = O == 16
+                       ? __builtin_amdgcn_permlane16_swap(u, u, false, false)
+                       : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return {__uint_as_float(r[0]), __uint_as_float(r[1])};
+  }
+}
+
+// Reductions over the wave, in every lane.
+template <typename Op>
+__device__ __forceinline__ float wave_reduce(float v, Op op) {
+  Pair p = lanes<1>(v);
+  v = op(p.x, p.y);
+  p = lanes<2>(v);
+  v = op(p.x, p.y);
+  p = lanes<4>(v);
+  v = op(p.x, p.y);
+  p = lanes<8>(v);
+  v = op(p.x, p.y);
+  p = lanes<16>(v);
+  v = op(p.x, p.y);
+  p = lanes<32>(v);
+  return op(p.x, p.y);
+}
 template <typename A, typename Op>
 __device__ __forceinline__ A wave_reduce(A v, Op op) {
 #pragma unroll
@@ -139,17 +182,16 @@ __device__ __forceinline__ A block_reduce(A v, Op op, A* scratch) {
   return v;
 }
 
-// The block's maximum in every thread, NaN if there is one; NT / 64 is a power
-// of two. One barrier: `scratch` must not be written again before the next.
+// The block's maximum in every thread, NaN if there is one. One barrier:
+// `scratch` must not be written again before the next.
 template <int NT>
 __device__ __forceinline__ float block_max(float v, float* scratch) {
-  constexpr int W = NT / 64;
   v = wave_reduce(v, MaxNan{});
   if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
   __syncthreads();
-  v = scratch[threadIdx.x & (W - 1)];
+  v = scratch[0];
 #pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) v = MaxNan{}(v, __shfl_xor(v, o));
+  for (int i = 1; i < NT / 64; ++i) v = MaxNan{}(v, scratch[i]);
   return v;
 }
 

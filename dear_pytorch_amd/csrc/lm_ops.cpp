@@ -247,10 +247,9 @@ void check_logits(const Tensor& t, const char* name) {
                     "tokens");
 }
 
-// What the slices of rows leave for each other, where a row has more than one
+// What the slices of rows leave for the kernel that joins them
 Tensor slice_records(const Tensor& logits, const LogitRows& z) {
   const int64_t n = dear_logit_slices(type_code(logits, "logits"), z.width);
-  if (n == 1) return Tensor();
   return at::empty({z.rows * n, dear_slice_bytes()},
                    logits.options().dtype(at::kByte));
 }
@@ -278,7 +277,7 @@ variable_list logprobs_forward(const Tensor& logits, const Tensor& tokens,
     const int type = type_code(logits, "logits");
     const Tensor part = slice_records(logits, z);
     Tensor lists;
-    if (top && part.defined())
+    if (top)
       lists = at::empty({part.size(0), top}, logits.options().dtype(at::kLong));
     check_launch(dear_logprobs_fwd(
         stream_of(logits), type, data(z.t),

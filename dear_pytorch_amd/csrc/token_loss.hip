@@ -14,11 +14,10 @@
 //   (p_t = 0) the term of q_t is left out of loss and W.
 //
 // Forward: a block takes a slice of one row into registers, 16 bytes a load,
-// and passes over it there: the maximum, then the sums, then the top. A
-// vocabulary of up to 32768 fp32 or 65536 16-bit tokens is one slice, and the
-// block finishes the row; longer rows leave a record for each slice, and a
-// second kernel joins them. Backward: one pass, elementwise, then the few
-// named tokens again.
+// passes over it there (the maximum, then the sums, then the top) and leaves a
+// record; a second kernel joins a row's records, a wave for each row, and does
+// the fp64 arithmetic, whose registers would cost the first one half of its
+// waves. Backward: one pass, elementwise, then the few named tokens again.
 //
 // Precision: exp(t) is exp2((z - m) c) with c = log2(e) / T: the difference is
 // taken first, so that it is 0 for the largest element and small errors stay
@@ -54,6 +53,10 @@ __device__ __forceinline__ uint64_t candidate(float z, int id) {
   return (uint64_t)order_key(z) << 32 | ~(uint32_t)id;
 }
 __device__ __forceinline__ int id_of(uint64_t c) { return ~(uint32_t)c; }
+__device__ __forceinline__ float logit_of(uint64_t c) {
+  const uint32_t key = (uint32_t)(c >> 32);
+  return __uint_as_float(key >> 31 ? key ^ 0x80000000u : ~key);
+}
 
 // What a row leaves for its backward pass: p_j = exp2((z_j - m) c) inv_s.
 // inv_s == 0: the row was not looked at, its gradient is zero.
@@ -92,19 +95,32 @@ struct Slice {
   __device__ __forceinline__ float at(int v, int j) const {
     return elem<T>(raw[v], j);
   }
-  // tokens [0, len) of z; what lies behind is -inf, which adds nothing
+  // tokens [0, len) of z; what lies behind is -inf, which adds nothing. One
+  // 32-bit offset serves all loads, with the row's address in scalar registers.
   __device__ __forceinline__ void load(const T* z, int len) {
+    const uint32_t mine = threadIdx.x * 16u;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int i = first(v);
-      if (i + E <= len) {
-        raw[v] = load16(z + i);
+      const char* p = reinterpret_cast<const char*>(z + v * NT * E);
+      if ((v + 1) * NT * E <= len) {          // the same for all threads
+        raw[v] = load16(reinterpret_cast<const T*>(p + mine));
       } else {
+        const int i = first(v);
         raw[v] = minus_inf<T>();
-        for (int j = 0; j < E; ++j)
-          if (i + j < len) put(raw[v], j, z[i + j]);
+        if (i + E <= len) {
+          raw[v] = load16(reinterpret_cast<const T*>(p + mine));
+        } else {
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (i + j < len) put(raw[v], j, z[i + j]);
+        }
       }
     }
+  }
+  // The compiler is not to keep the fp32 values of one pass for the next: they
+  // would take twice the registers, and half of the waves.
+  __device__ __forceinline__ void fresh(int v) {
+    asm volatile("" : "+v"(raw[v]));
   }
   // NaN if the thread holds one
   __device__ __forceinline__ float max() {
@@ -126,7 +142,7 @@ struct Slice {
 // ids. For rows whose order the quick way cannot use: NaN, or very many equal
 // elements. 31 + 32 passes over the slice.
 template <typename T, int NT>
-__device__ void bisect_top(const T* z, int len, int base, int k,
+__device__ __noinline__ void bisect_top(const T* z, int len, int base, int k,
                            uint64_t* found, int* count, int* scratch) {
   uint32_t key = 0;
   for (int bit = 31; bit >= 0; --bit) {
@@ -161,18 +177,22 @@ __device__ void bisect_top(const T* z, int len, int base, int k,
 }
 
 // Lanes' values in falling order (bitonic, 21 exchanges).
-__device__ __forceinline__ float wave_sort(float v) {
+template <int Size, int O>
+__device__ __forceinline__ float exchange(float v) {
   const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-    for (int o = size >> 1; o > 0; o >>= 1) {
-      const float w = __shfl_xor(v, o);
-      const bool larger = ((lane & o) == 0) == ((lane & size) == 0 ||
-                                                size == 64);
-      v = larger ? fmaxf(v, w) : fminf(v, w);
-    }
-  return v;
+  const Pair p = lanes<O>(v);
+  const bool larger = ((lane & O) == 0) == ((lane & Size) == 0);
+  v = larger ? fmaxf(p.x, p.y) : fminf(p.x, p.y);
+  if constexpr (O > 1) return exchange<Size, O / 2>(v);
+  else return v;
+}
+__device__ __forceinline__ float wave_sort(float v) {
+  v = exchange<2, 1>(v);
+  v = exchange<4, 2>(v);
+  v = exchange<8, 4>(v);
+  v = exchange<16, 8>(v);
+  v = exchange<32, 16>(v);
+  return exchange<64, 32>(v);
 }
 
 // The k best of a slice into found[0..n), in no order; every thread gets n.
@@ -180,7 +200,7 @@ __device__ __forceinline__ float wave_sort(float v) {
 // of the waves' such maxima of threads: k elements at least reach it, and
 // about k ln(waves) do if the row is in no order. Only those are collected.
 template <typename T, int NT, int NV>
-__device__ int slice_top(const Slice<T, NT, NV>& s, const T* z, int len,
+__device__ int slice_top(Slice<T, NT, NV>& s, const T* z, int len,
                          int base, int k, float mine, bool has_nan,
                          uint64_t* found, int* count, float* wave_floor,
                          int* scratch) {
@@ -197,12 +217,13 @@ __device__ int slice_top(const Slice<T, NT, NV>& s, const T* z, int len,
     if (lane == 0) wave_floor[wave] = bar;
     if (threadIdx.x == 0) *count = 0;
     __syncthreads();
-    bar = wave_floor[lane & (W - 1)];
+    bar = wave_floor[0];
 #pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) bar = fminf(bar, __shfl_xor(bar, o));
+    for (int i = 1; i < W; ++i) bar = fminf(bar, wave_floor[i]);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       if (!(s.vmax[v] >= bar)) continue;
+      s.fresh(v);
       const int i = Slice<T, NT, NV>::first(v);
 #pragma unroll
       for (int j = 0; j < kVec<T>; ++j) {
@@ -245,46 +266,42 @@ struct Bits {
 };
 
 // Adds up one slice against the maximum m (not NaN, finite). ENT: e2 too.
-// Results in the first wave's lane 0.
+// Results in every thread of the first wave.
 template <typename T, int NT, int NV, bool ENT, typename B>
-__device__ __forceinline__ Sums slice_sums(const Slice<T, NT, NV>& s, B bits,
-                                           float m, float mine, Factor f,
+__device__ __forceinline__ Sums slice_sums(Slice<T, NT, NV>& s, B bits,
+                                           float m, Factor f,
                                            float (*scratch)[6]) {
   constexpr int W = NT / 64, E = kVec<T>;
   float rest = 0.f, e2 = 0.f, in = 0.f, n = 0.f, n_in = 0.f;
-  auto plain = [&](int v) {
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const float y = (s.at(v, j) - m) * f.c;
-      const float e = __builtin_amdgcn_exp2f(y);
-      rest += e;
-      if constexpr (ENT) e2 = fmaf(e, fmaxf(y, -256.f), e2);  // 0 for -inf
-    }
-  };
-  auto careful = [&](int v, uint32_t named) {
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const float z = s.at(v, j);
-      const bool inside = B::kTail && (named >> j & 1);
-      if (z == m) {
-        if (inside) n_in += 1.f;
-        else n += 1.f;
-      } else {
-        const float y = (z - m) * f.c;
-        const float e = __builtin_amdgcn_exp2f(y);
-        if (inside) in += e;
-        else rest += e;
-        if constexpr (ENT) e2 = fmaf(e, fmaxf(y, -256.f), e2);
-      }
-    }
-  };
-  const bool owner = mine == m;          // holds an element equal to m
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
+    s.fresh(v);
     uint32_t named = 0;
     if constexpr (B::kTail) named = bits.named[v * NT + threadIdx.x];
-    if (owner || named) careful(v, named);
-    else plain(v);
+    if (s.vmax[v] != m && named == 0) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float y = (s.at(v, j) - m) * f.c;
+        const float e = __builtin_amdgcn_exp2f(y);
+        rest += e;
+        if constexpr (ENT) e2 = fmaf(e, fmaxf(y, -256.f), e2);  // 0 for -inf
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float z = s.at(v, j), y = (z - m) * f.c;
+        const float e = __builtin_amdgcn_exp2f(y);
+        const bool inside = B::kTail && (named >> j & 1);
+        if (z == m) {
+          if (inside) n_in += 1.f;
+          else n += 1.f;
+        } else {
+          if (inside) in += e;
+          else rest += e;
+          if constexpr (ENT) e2 = fmaf(e, fmaxf(y, -256.f), e2);
+        }
+      }
+    }
   }
   rest = wave_reduce(rest, Add{});
   n = wave_reduce(n, Add{});
@@ -293,34 +310,27 @@ __device__ __forceinline__ Sums slice_sums(const Slice<T, NT, NV>& s, B bits,
     in = wave_reduce(in, Add{});
     n_in = wave_reduce(n_in, Add{});
   }
-  const int lane = threadIdx.x & 63;
-  if (lane == 0) {
+  if ((threadIdx.x & 63) == 0) {
     float* p = scratch[threadIdx.x >> 6];
     p[0] = rest; p[1] = n; p[2] = e2; p[3] = in; p[4] = n_in;
   }
   __syncthreads();
   Sums r = {};
   if (threadIdx.x < 64) {
-    const float* p = scratch[lane & (W - 1)];
-    r.rest = p[0];
-    r.n = p[1];
-    r.e2 = p[2];
-    r.in = p[3];
-    r.n_in = p[4];
-#pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) {
-      r.rest += __shfl_xor(r.rest, o);
-      r.n += __shfl_xor(r.n, o);
-      if constexpr (ENT) r.e2 += __shfl_xor(r.e2, o);
+    for (int i = 0; i < W; ++i) {
+      const float* p = scratch[i];
+      r.rest += p[0];
+      r.n += p[1];
+      if constexpr (ENT) r.e2 += p[2];
       if constexpr (B::kTail) {
-        r.in += __shfl_xor(r.in, o);
-        r.n_in += __shfl_xor(r.n_in, o);
+        r.in += p[3];
+        r.n_in += p[4];
       }
     }
-    r.m = m;
     // exp2(y c_exact / c) of every element, to first order (2^-25 squared)
     if constexpr (ENT) r.rest += (f.exact / (double)f.c - 1.0) * kLn2 * r.e2;
   }
+  r.m = m;
   return r;
 }
 
@@ -372,127 +382,87 @@ struct LogprobArgs {
   float *logprob, *entropy, *top_lp;
   int64_t* top_ids;
   RowStats* stats;
-  Sums* part;                // [rows][slices], of more than one slice
+  Sums* part;                // [rows][slices]
   uint64_t* lists;           // [rows][slices][k], best first, 0: no such one
 };
 
-// One thread: everything of a row but its top; returns log s (NaN: bad).
-template <typename T>
-__device__ __forceinline__ double finish_logprob(const LogprobArgs& a,
-                                                 int64_t row, const T* z,
-                                                 const Sums& s) {
-  const float m = (float)s.m;
-  const bool bad = no_distribution(m);
-  const double others = s.rest + (s.n - 1.0), sum = 1.0 + others;
-  const double log_s = bad ? NAN : log1p(others);
-  const double h = log_s - kLn2 * s.e2 / sum;
-  a.entropy[row] = (float)h;
-  if (a.tokens) {
-    const int64_t token = a.tokens[row];
-    const bool known = token >= 0 && token < a.V;
-    a.logprob[row] =
-        known ? (float)(((double)to_f(z[token]) - s.m) * a.inv_t - log_s)
-              : NAN;
-  }
-  if (a.stats)
-    a.stats[row] = {m, bad ? NAN : (float)(1.0 / sum), (float)(h - log_s),
-                    0.f};
-  return log_s;
-}
-
-__device__ __forceinline__ void skip_logprob(const LogprobArgs& a,
-                                             int64_t row) {
-  if (threadIdx.x == 0) {
-    a.logprob[row] = 0.f;
-    a.entropy[row] = 0.f;
-    if (a.stats) a.stats[row] = {0.f, 0.f, 0.f, 0.f};
-  }
-  for (int i = threadIdx.x; i < a.k; i += blockDim.x) {
-    a.top_lp[row * a.k + i] = -INFINITY;
-    a.top_ids[row * a.k + i] = -1;
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void put_top(const LogprobArgs& a, int64_t row,
-                                        const T* z, int rank, int id, double m,
-                                        double log_s) {
-  a.top_ids[row * a.k + rank] = id;
-  a.top_lp[row * a.k + rank] =
-      (float)(((double)to_f(z[id]) - m) * a.inv_t - log_s);
-}
-
 template <typename T, int NT, int NV, bool TOP>
-__global__ __launch_bounds__(NT) void logprobs_slice_kernel(
+__global__ __launch_bounds__(NT, 4) void logprobs_slice_kernel(
     const T* __restrict__ logits, const LogprobArgs a) {
   __shared__ float wave_max[NT / 64], wave_floor[NT / 64];
   __shared__ float sums[NT / 64][6];
   __shared__ int scratch[NT / 64];
   __shared__ uint64_t found[TOP ? kCandidates : 1];
-  __shared__ double log_sum;
   __shared__ int count;
   const int64_t work = a.rows * a.slices;
   for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
     const int64_t row = a.slices == 1 ? w : w / a.slices;
     const int base = (int)(w - row * a.slices) * a.per_slice;
-    if (a.tokens && a.tokens[row] == a.ignore) {
-      if (base == 0) skip_logprob(a, row);
-      continue;
-    }
-    const T* z = logits + row * a.zs;
+    if (a.tokens && a.tokens[row] == a.ignore) continue;
+    const T* z = logits + row * a.zs + base;
     const int len = min(a.per_slice, a.V - base);
     Slice<T, NT, NV> s;
-    s.load(z + base, len);
+    s.load(z, len);
     const float mine = s.max();
     const float m = block_max<NT>(mine, wave_max);
     Sums r = {};
     if (!no_distribution(m))
-      r = slice_sums<T, NT, NV, true>(s, NoBits{}, m, mine, a.f, sums);
+      r = slice_sums<T, NT, NV, true>(s, NoBits{}, m, a.f, sums);
     r.m = m;
-    if (threadIdx.x == 0) {
-      if (a.slices == 1) log_sum = finish_logprob(a, row, z, r);
-      else a.part[w] = r;
-    }
+    if (threadIdx.x == 0) a.part[w] = r;
     if constexpr (TOP) {
       const int k = min(a.k, len);
-      const int n = slice_top(s, z + base, len, base, k, mine, m != m, found,
-                              &count, wave_floor, scratch);
-      if (a.slices == 1) {
-        const double log_s = log_sum;    // slice_top has synchronised
-        ranked<NT>(found, n, k, [&](int rank, uint64_t c) {
-          put_top(a, row, z, rank, id_of(c), (double)m, log_s);
-        });
-      } else {
-        uint64_t* list = a.lists + w * a.k;
-        ranked<NT>(found, n, k, [&](int rank, uint64_t c) { list[rank] = c; });
-        for (int i = k + threadIdx.x; i < a.k; i += NT) list[i] = 0;
-      }
+      const int n = slice_top(s, z, len, base, k, mine, m != m, found, &count,
+                              wave_floor, scratch);
+      uint64_t* list = a.lists + w * a.k;
+      ranked<NT>(found, n, k, [&](int rank, uint64_t c) { list[rank] = c; });
+      for (int i = k + threadIdx.x; i < a.k; i += NT) list[i] = 0;
     }
     __syncthreads();                     // before the arrays are used again
   }
 }
 
-// Rows of more than one slice: a block of 256 joins the records of one row.
+// Four rows to a block, a wave each.
 template <typename T>
-__global__ __launch_bounds__(256) void logprobs_join_kernel(
+__global__ __launch_bounds__(256) void logprobs_finish_kernel(
     const T* __restrict__ logits, const LogprobArgs a) {
-  __shared__ double shared[2];
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    if (a.tokens && a.tokens[row] == a.ignore) continue;
-    const T* z = logits + row * a.zs;
-    if (threadIdx.x < 64) {
-      const Sums s = join_sums(a.part + row * a.slices, a.slices, a.f);
-      if (threadIdx.x == 0) {
-        shared[0] = finish_logprob(a, row, z, s);
-        shared[1] = s.m;
+  const int lane = threadIdx.x & 63;
+  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+       row < a.rows; row += (int64_t)gridDim.x * 4) {
+    const int64_t token = a.tokens ? a.tokens[row] : -1;
+    if (a.tokens && token == a.ignore) {
+      if (lane == 0) {
+        a.logprob[row] = 0.f;
+        a.entropy[row] = 0.f;
+        if (a.stats) a.stats[row] = {0.f, 0.f, 0.f, 0.f};
       }
+      for (int i = lane; i < a.k; i += 64) {
+        a.top_lp[row * a.k + i] = -INFINITY;
+        a.top_ids[row * a.k + i] = -1;
+      }
+      continue;
     }
-    __syncthreads();
-    const double log_s = shared[0], m = shared[1];
+    const float at = token >= 0 && token < a.V
+                         ? to_f(logits[row * a.zs + token])
+                         : NAN;
+    const Sums s = join_sums(a.part + row * a.slices, a.slices, a.f);
+    const float m = (float)s.m;
+    const bool bad = no_distribution(m);
+    const double others = s.rest + (s.n - 1.0), sum = 1.0 + others;
+    const double log_s = bad ? NAN : log1p(others);
+    const double h = log_s - kLn2 * s.e2 / sum;
+    if (lane == 0) {
+      a.entropy[row] = (float)h;
+      if (a.tokens)
+        a.logprob[row] = (float)(((double)at - s.m) * a.inv_t - log_s);
+      if (a.stats)
+        a.stats[row] = {m, bad ? NAN : (float)(1.0 / sum), (float)(h - log_s),
+                        0.f};
+    }
     // the place of a candidate: its place in its own list, and how many of
     // each other list are better
     const uint64_t* lists = a.lists + row * a.slices * a.k;
-    for (int64_t i = threadIdx.x; i < a.slices * a.k; i += 256) {
+    for (int64_t i = lane; i < a.slices * a.k; i += 64) {
       const uint64_t mine = lists[i];
       if (mine == 0) continue;
       const int64_t own = i / a.k;
@@ -508,9 +478,12 @@ __global__ __launch_bounds__(256) void logprobs_join_kernel(
         }
         rank += lo;
       }
-      if (rank < a.k) put_top(a, row, z, (int)rank, id_of(mine), m, log_s);
+      if (rank < a.k) {
+        a.top_ids[row * a.k + rank] = id_of(mine);
+        a.top_lp[row * a.k + rank] =
+            (float)(((double)logit_of(mine) - s.m) * a.inv_t - log_s);
+      }
     }
-    __syncthreads();
   }
 }
 
@@ -528,78 +501,96 @@ struct DistillArgs {
   Sums* part;
 };
 
-// Whole block, of 256 threads or more; s: in every thread.
-template <typename T, bool TAIL>
-__device__ void finish_distill(const DistillArgs& a, int64_t row, const T* z,
-                               const Sums& s, int64_t id, double* scratch,
-                               double* shares, int64_t* named) {
-  const int tid = threadIdx.x, k = a.k;
-  const bool present = id >= 0;
-  const float lp = present ? a.teacher[row * k + tid] : -INFINITY;
-  double q, rest = 0.0;
+// A row's entries, two to a lane of the wave that finishes the row: loaded
+// before the row's sums are known.
+struct Entries {
+  int64_t id[2];
+  float lp[2], z[2];       // the teacher's, and the student's logit
+  template <typename T>
+  __device__ __forceinline__ void load(const DistillArgs& a, int64_t row,
+                                       const T* logits) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = (threadIdx.x & 63) + 64 * e;
+      id[e] = i < a.k ? a.ids[row * a.k + i] : -1;
+      lp[e] = id[e] >= 0 ? a.teacher[row * a.k + i] : -INFINITY;
+      // an id outside of the vocabulary: NaN
+      z[e] = id[e] < 0 ? 0.f : id[e] < a.V ? to_f(logits[id[e]]) : NAN;
+    }
+  }
+};
+
+// One wave. `ids`, `shares`: k of each in LDS, for this wave alone.
+template <bool TAIL>
+__device__ void finish_distill(const DistillArgs& a, int64_t row,
+                               const Sums& s, const Entries& t, int64_t* ids,
+                               double* shares) {
+  const int lane = threadIdx.x & 63;
+  double q[2], rest = 0.0;
   if constexpr (TAIL) {
-    q = exp((double)lp);
-    const double left = 1.0 - block_reduce(q, Add{}, scratch);
+    q[0] = exp((double)t.lp[0]);
+    q[1] = exp((double)t.lp[1]);
+    const double left = 1.0 - wave_reduce(q[0] + q[1], Add{});
     rest = left <= 0.0 ? 0.0 : left;
   } else {
-    const float top = block_reduce(lp, MaxNan{},
-                                   reinterpret_cast<float*>(scratch));
-    q = top == -INFINITY ? 0.0 : exp((double)lp - (double)top);
-    const double sum = block_reduce(q, Add{}, scratch);
-    q = sum == 0.0 ? 0.0 : q / sum;
+    const float top = wave_reduce(MaxNan{}(t.lp[0], t.lp[1]), MaxNan{});
+    const bool none = top == -INFINITY;
+    q[0] = none ? 0.0 : exp((double)t.lp[0] - (double)top);
+    q[1] = none ? 0.0 : exp((double)t.lp[1] - (double)top);
+    const double sum = wave_reduce(q[0] + q[1], Add{});
+    if (sum != 0.0) {
+      q[0] /= sum;
+      q[1] /= sum;
+    }
   }
   const float m = (float)s.m;
   const double outside = s.n + s.rest;
   const double others = (s.rest + s.in) + ((s.n + s.n_in) - 1.0);
   const double sum = 1.0 + others, log_s = log1p(others);
-  double term = 0.0;
-  if (id >= a.V) term = NAN;                 // no such token
-  else if (present && q != 0.0)
-    term = q * (log(q) - (((double)to_f(z[id]) - s.m) / a.t - log_s));
-  double total = block_reduce(term, Add{}, scratch);
-  double share = block_reduce(q, Add{}, scratch), shift = 0.0;
+  double total = 0.0;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (t.z[e] != t.z[e])                    // no such token, or a NaN
+      total = NAN;
+    else if (q[e] != 0.0)
+      total += q[e] * (log(q[e]) - (((double)t.z[e] - s.m) / a.t - log_s));
+  total = wave_reduce(total, Add{});
+  double share = wave_reduce(q[0] + q[1], Add{}), shift = 0.0;
   if (TAIL && rest != 0.0 && outside > 0.0) {
     share += rest;
     total += rest * (log(rest) - (log(outside) - log_s));
     shift = rest * sum / outside;
   }
   if (no_distribution(m)) total = NAN;
-  if (tid == 0) a.loss[row] = (float)(total * a.t * a.t);
-  if (a.stats) {
-    if (tid == 0)
-      a.stats[row] = {m, total != total ? NAN : (float)(1.0 / sum),
-                      (float)share, (float)(share - shift)};
-    // an id that is named more than once: each entry gets the sum
-    if (tid < k) {
-      shares[tid] = q;
-      named[tid] = id;
+  if (lane == 0) a.loss[row] = (float)(total * a.t * a.t);
+  if (!a.stats) return;
+  if (lane == 0)
+    a.stats[row] = {m, total != total ? NAN : (float)(1.0 / sum),
+                    (float)share, (float)(share - shift)};
+  // an id that is named more than once: each of its entries gets the sum
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (lane + 64 * e < a.k) {
+      ids[lane + 64 * e] = t.id[e];
+      shares[lane + 64 * e] = q[e];
     }
-    __syncthreads();
-    if (tid < k) {
-      double all = 0.0;
-      for (int i = 0; i < k; ++i) all += named[i] == id ? shares[i] : 0.0;
-      a.q_out[row * k + tid] = (float)all;
-    }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (lane + 64 * e >= a.k) break;
+    double all = 0.0;
+    for (int i = 0; i < a.k; ++i) all += ids[i] == t.id[e] ? shares[i] : 0.0;
+    a.q_out[row * a.k + lane + 64 * e] = (float)all;
   }
-}
-
-__device__ __forceinline__ void skip_distill(const DistillArgs& a,
-                                             int64_t row) {
-  if (threadIdx.x == 0) {
-    a.loss[row] = 0.f;
-    if (a.stats) a.stats[row] = {0.f, 0.f, 0.f, 0.f};
-  }
-  if (a.stats && threadIdx.x < a.k) a.q_out[row * a.k + threadIdx.x] = 0.f;
 }
 
 template <typename T, int NT, int NV, bool TAIL>
-__global__ __launch_bounds__(NT) void distill_slice_kernel(
+__global__ __launch_bounds__(NT, 4) void distill_slice_kernel(
     const T* __restrict__ logits, const DistillArgs a) {
   __shared__ float wave_max[NT / 64];
   __shared__ float sums[NT / 64][6];
-  __shared__ double scratch[NT / 64], shares[kMaxTop];
-  __shared__ int64_t named[kMaxTop];
-  __shared__ Sums whole;
   __shared__ uint32_t bits[TAIL ? NT * NV / 4 : 1];
   const int64_t work = a.rows * a.slices;
   const int tid = threadIdx.x;
@@ -609,14 +600,10 @@ __global__ __launch_bounds__(NT) void distill_slice_kernel(
     const int64_t id = tid < a.k ? a.ids[row * a.k + tid] : -1;
     if constexpr (TAIL)
       for (int i = tid; i < NT * NV / 4; i += NT) bits[i] = 0;
-    if (!__syncthreads_or(id >= 0)) {
-      if (base == 0) skip_distill(a, row);
-      continue;
-    }
-    const T* z = logits + row * a.zs;
+    if (!__syncthreads_or(id >= 0)) continue;
     const int len = min(a.per_slice, a.V - base);
     Slice<T, NT, NV> s;
-    s.load(z + base, len);
+    s.load(logits + row * a.zs + base, len);
     if constexpr (TAIL) {
       const int64_t at = id - base;
       if (at >= 0 && at < len) {
@@ -631,41 +618,38 @@ __global__ __launch_bounds__(NT) void distill_slice_kernel(
     if (!no_distribution(m)) {
       if constexpr (TAIL)
         r = slice_sums<T, NT, NV, false>(
-            s, Bits{reinterpret_cast<const uint8_t*>(bits)}, m, mine, a.f,
-            sums);
+            s, Bits{reinterpret_cast<const uint8_t*>(bits)}, m, a.f, sums);
       else
-        r = slice_sums<T, NT, NV, false>(s, NoBits{}, m, mine, a.f, sums);
+        r = slice_sums<T, NT, NV, false>(s, NoBits{}, m, a.f, sums);
     }
     r.m = m;
-    if (a.slices == 1) {
-      if (tid == 0) whole = r;
-      __syncthreads();
-      finish_distill<T, TAIL>(a, row, z, whole, id, scratch, shares, named);
-    } else if (tid == 0) {
-      a.part[w] = r;
-    }
+    if (tid == 0) a.part[w] = r;
     __syncthreads();
   }
 }
 
+// Four rows to a block, a wave each.
 template <typename T, bool TAIL>
-__global__ __launch_bounds__(256) void distill_join_kernel(
+__global__ __launch_bounds__(256) void distill_finish_kernel(
     const T* __restrict__ logits, const DistillArgs a) {
-  __shared__ double scratch[4], shares[kMaxTop];
-  __shared__ int64_t named[kMaxTop];
-  __shared__ Sums whole;
-  const int tid = threadIdx.x;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const int64_t id = tid < a.k ? a.ids[row * a.k + tid] : -1;
-    if (!__syncthreads_or(id >= 0)) continue;
-    if (tid < 64) {
-      const Sums s = join_sums(a.part + row * a.slices, a.slices, a.f);
-      if (tid == 0) whole = s;
+  __shared__ double shares[4][kMaxTop];
+  __shared__ int64_t named[4][kMaxTop];
+  const int wave = threadIdx.x >> 6;
+  for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < a.rows;
+       row += (int64_t)gridDim.x * 4) {
+    Entries t;
+    t.load(a, row, logits + row * a.zs);
+    if (!__any(t.id[0] >= 0 || t.id[1] >= 0)) {
+      const int lane = threadIdx.x & 63;
+      if (lane == 0) a.loss[row] = 0.f;
+      if (a.stats) {
+        if (lane == 0) a.stats[row] = {0.f, 0.f, 0.f, 0.f};
+        for (int i = lane; i < a.k; i += 64) a.q_out[row * a.k + i] = 0.f;
+      }
+      continue;
     }
-    __syncthreads();
-    finish_distill<T, TAIL>(a, row, logits + row * a.zs, whole, id, scratch,
-                            shares, named);
-    __syncthreads();
+    const Sums s = join_sums(a.part + row * a.slices, a.slices, a.f);
+    finish_distill<TAIL>(a, row, s, t, named[wave], shares[wave]);
   }
 }
 
@@ -826,28 +810,26 @@ Factor exp2_factor(double t) {
 }
 
 // Threads and 16-byte vectors of a slice: the smallest block that holds the
-// row, up to 8192 vectors; longer rows in equal slices.
+// row, up to 4096 vectors; longer rows in equal slices.
 struct Cut {
-  int threads, vectors, per_slice;
+  int vectors, per_slice;
   int64_t slices;
 };
 
 Cut cut_row(int V, int per_vector) {
   const int64_t vecs = (V + per_vector - 1) / per_vector;
-  const int64_t few = (vecs + 8191) / 8192;
+  const int64_t few = (vecs + 4095) / 4096;
   const int64_t each = (vecs + few - 1) / few;
   const int64_t slices = (vecs + each - 1) / each;     // none of them empty
-  const int threads = each <= 1024 ? 256 : 1024;
-  const int vectors = each <= 256 ? 1 : each <= 1024 || each <= 4096 ? 4 : 8;
-  return {threads, vectors, (int)(each * per_vector), slices};
+  const int vectors = each <= 256 ? 1 : each <= 1024 ? 4 : 8;
+  return {vectors, (int)(each * per_vector), slices};
 }
 
 template <typename F>
 void with_cut(const Cut& c, F f) {
-  if (c.threads == 256 && c.vectors == 1) f(Int<256>{}, Int<1>{});
-  else if (c.threads == 256) f(Int<256>{}, Int<4>{});
-  else if (c.vectors == 4) f(Int<1024>{}, Int<4>{});
-  else f(Int<1024>{}, Int<8>{});
+  if (c.vectors == 1) f(Int<256>{}, Int<1>{});
+  else if (c.vectors == 4) f(Int<256>{}, Int<4>{});
+  else f(Int<512>{}, Int<8>{});
 }
 
 template <typename F>
@@ -861,8 +843,7 @@ int per_vector(int type) { return type == kF32 ? 4 : 8; }
 
 }  // namespace
 
-// Slices of a row, and bytes of the record that each leaves where there is
-// more than one.
+// Slices of a row, and bytes of the record that each leaves.
 int64_t dear_logit_slices(int type, int V) {
   return cut_row(V, per_vector(type)).slices;
 }
@@ -890,9 +871,9 @@ int dear_logprobs_fwd(hipStream_t st, int type, const void* logits, int64_t zs,
         hipLaunchKernelGGL((logprobs_slice_kernel<T, NT, NV, false>), grid,
                            block, 0, st, (const T*)logits, a);
     });
-    if (cut.slices > 1)
-      hipLaunchKernelGGL((logprobs_join_kernel<T>), dim3(grid_for(rows)),
-                         dim3(256), 0, st, (const T*)logits, a);
+    hipLaunchKernelGGL((logprobs_finish_kernel<T>),
+                       dim3(grid_for((rows + 3) / 4)), dim3(256), 0, st,
+                       (const T*)logits, a);
   });
   return (int)hipGetLastError();
 }
@@ -942,16 +923,13 @@ int dear_distill_fwd(hipStream_t st, int type, bool tail, const void* logits,
         hipLaunchKernelGGL((distill_slice_kernel<T, NT, NV, false>), grid,
                            block, 0, st, (const T*)logits, a);
     });
-    if (cut.slices > 1) {
-      if (tail)
-        hipLaunchKernelGGL((distill_join_kernel<T, true>),
-                           dim3(grid_for(rows)), dim3(256), 0, st,
-                           (const T*)logits, a);
-      else
-        hipLaunchKernelGGL((distill_join_kernel<T, false>),
-                           dim3(grid_for(rows)), dim3(256), 0, st,
-                           (const T*)logits, a);
-    }
+    const dim3 rest(grid_for((rows + 3) / 4));
+    if (tail)
+      hipLaunchKernelGGL((distill_finish_kernel<T, true>), rest, dim3(256), 0,
+                         st, (const T*)logits, a);
+    else
+      hipLaunchKernelGGL((distill_finish_kernel<T, false>), rest, dim3(256), 0,
+                         st, (const T*)logits, a);
   });
   return (int)hipGetLastError();
 }
