@@ -112,6 +112,12 @@ struct Max {
     return fmaxf(a, b);
   }
 };
+struct Larger {
+  template <typename A>
+  __device__ __forceinline__ A operator()(A a, A b) const {
+    return a > b ? a : b;
+  }
+};
 // NaN wins: a row that holds one has to say so
 struct MaxNan {
   __device__ __forceinline__ float operator()(float a, float b) const {
@@ -144,6 +150,27 @@ __device__ __forceinline__ Pair lanes(float v) {
                        : __builtin_amdgcn_permlane32_swap(u, u, false, false);
     return {__uint_as_float(r[0]), __uint_as_float(r[1])};
   }
+}
+
+// What the lanes of a wave have written to LDS is seen by all of them.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ float sum_of(Pair p) { return p.x + p.y; }
+
+// The sum over the lanes below this one.
+__device__ __forceinline__ int wave_before(int v) {
+  const int lane = threadIdx.x & 63;
+  int s = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int w = __shfl_up(s, o);
+    if (lane >= o) s += w;
+  }
+  return s - v;
 }
 
 // Reductions over the wave, in every lane.

@@ -15,7 +15,7 @@ int dear_ln_bwd(hipStream_t, int, int, int, const void*, int64_t, const void*,
                 int64_t, const void*, int64_t, const void*, const float*,
                 const float*, void*, void*, void*, void*, float*, int, int64_t,
                 int);
-int64_t dear_logit_slices(int, int);
+int64_t dear_logit_slices(int, int64_t, int);
 int64_t dear_slice_bytes();
 int dear_logprobs_fwd(hipStream_t, int, const void*, int64_t, const int64_t*,
                       int64_t, int64_t, int, int, double, float*, float*,
@@ -249,7 +249,8 @@ void check_logits(const Tensor& t, const char* name) {
 
 // What the slices of rows leave for the kernel that joins them
 Tensor slice_records(const Tensor& logits, const LogitRows& z) {
-  const int64_t n = dear_logit_slices(type_code(logits, "logits"), z.width);
+  const int64_t n = dear_logit_slices(type_code(logits, "logits"), z.rows,
+                                      z.width);
   return at::empty({z.rows * n, dear_slice_bytes()},
                    logits.options().dtype(at::kByte));
 }

@@ -196,6 +196,7 @@ __device__ __forceinline__ float wave_sort(float v) {
 }
 
 // The k best of a slice into found[0..n), in no order; every thread gets n.
+// k is at most NT.
 // Each of NT / 64 waves has ceil(k / waves) elements that reach the smallest
 // of the waves' such maxima of threads: k elements at least reach it, and
 // about k ln(waves) do if the row is in no order. Only those are collected.
@@ -220,19 +221,30 @@ __device__ int slice_top(Slice<T, NT, NV>& s, const T* z, int len,
     bar = wave_floor[0];
 #pragma unroll
     for (int i = 1; i < W; ++i) bar = fminf(bar, wave_floor[i]);
+    // a bit for each element of the thread that reaches the bar; then one
+    // place for all of the wave's, and the values from memory again
+    constexpr int E = kVec<T>;
+    static_assert(NV * E <= 64, "a bit for each");
+    uint64_t mask = 0;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       if (!(s.vmax[v] >= bar)) continue;
       s.fresh(v);
-      const int i = Slice<T, NT, NV>::first(v);
+      uint32_t bits = 0;
 #pragma unroll
-      for (int j = 0; j < kVec<T>; ++j) {
-        const float x = s.at(v, j);
-        if (x >= bar && i + j < len) {
-          const int at = atomicAdd(count, 1);
-          if (at < kCandidates) found[at] = candidate(x, base + i + j);
-        }
-      }
+      for (int j = 0; j < E; ++j) bits |= s.at(v, j) >= bar ? 1u << j : 0u;
+      const int left = len - Slice<T, NT, NV>::first(v);
+      if (left < E) bits &= (1u << max(left, 0)) - 1u;
+      mask |= (uint64_t)bits << v * E;
+    }
+    const int mine_n = __popcll(mask), before = wave_before(mine_n);
+    int at = 0;
+    if (lane == 63) at = atomicAdd(count, before + mine_n);
+    at = __shfl(at, 63) + before;
+    for (; mask != 0 && at < kCandidates; mask &= mask - 1, ++at) {
+      const int b = __ffsll((unsigned long long)mask) - 1;
+      const int i = (b / E * NT + (int)threadIdx.x) * E + b % E;
+      found[at] = candidate(to_f(z[i]), base + i);
     }
     __syncthreads();
     const int n = *count;
@@ -243,15 +255,25 @@ __device__ int slice_top(Slice<T, NT, NV>& s, const T* z, int len,
   return k;
 }
 
-// Calls put(rank, candidate) for the k best of found[0..n).
+// Calls put(rank, candidate) for the k best of found[0..n): the rank is how
+// many are better, counted by 2^share lanes together.
 template <int NT, typename Put>
 __device__ __forceinline__ void ranked(const uint64_t* found, int n, int k,
                                        Put put) {
-  for (int i = threadIdx.x; i < n; i += NT) {
-    const uint64_t mine = found[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += found[j] > mine;
-    if (rank < k) put(rank, mine);
+  int share = 0;
+  while (share < 3 && (n << (share + 1)) <= NT) ++share;
+  const int sub = threadIdx.x & ((1 << share) - 1);
+  // whole waves go round together, for their lanes add up each other's counts
+  for (int first = 0; first < n; first += NT >> share) {
+    const int i = first + ((int)threadIdx.x >> share);
+    const uint64_t mine = i < n ? found[i] : 0;
+    float better = 0.f;
+    for (int j = sub; j < n; j += 1 << share)
+      better += found[j] > mine ? 1.f : 0.f;
+    if (share > 0) better = sum_of(lanes<1>(better));
+    if (share > 1) better = sum_of(lanes<2>(better));
+    if (share > 2) better = sum_of(lanes<4>(better));
+    if (i < n && sub == 0 && better < (float)k) put((int)better, mine);
   }
 }
 
@@ -338,6 +360,7 @@ __device__ __forceinline__ Sums slice_sums(Slice<T, NT, NV>& s, B bits,
 // of -inf alone adds nothing.
 __device__ __forceinline__ Sums join_sums(const Sums* part, int64_t ns,
                                           Factor f) {
+  if (ns == 1) return part[0];
   const int lane = threadIdx.x & 63;
   float m = -INFINITY;
   for (int64_t i = lane; i < ns; i += 64)
@@ -387,7 +410,7 @@ struct LogprobArgs {
 };
 
 template <typename T, int NT, int NV, bool TOP>
-__global__ __launch_bounds__(NT, 4) void logprobs_slice_kernel(
+__global__ __launch_bounds__(NT, 6) void logprobs_slice_kernel(
     const T* __restrict__ logits, const LogprobArgs a) {
   __shared__ float wave_max[NT / 64], wave_floor[NT / 64];
   __shared__ float sums[NT / 64][6];
@@ -426,9 +449,11 @@ __global__ __launch_bounds__(NT, 4) void logprobs_slice_kernel(
 template <typename T>
 __global__ __launch_bounds__(256) void logprobs_finish_kernel(
     const T* __restrict__ logits, const LogprobArgs a) {
-  const int lane = threadIdx.x & 63;
-  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-       row < a.rows; row += (int64_t)gridDim.x * 4) {
+  constexpr int kHeld = 1024;
+  __shared__ uint64_t held[4][kHeld];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < a.rows;
+       row += (int64_t)gridDim.x * 4) {
     const int64_t token = a.tokens ? a.tokens[row] : -1;
     if (a.tokens && token == a.ignore) {
       if (lane == 0) {
@@ -459,31 +484,60 @@ __global__ __launch_bounds__(256) void logprobs_finish_kernel(
         a.stats[row] = {m, bad ? NAN : (float)(1.0 / sum), (float)(h - log_s),
                         0.f};
     }
-    // the place of a candidate: its place in its own list, and how many of
-    // each other list are better
     const uint64_t* lists = a.lists + row * a.slices * a.k;
-    for (int64_t i = lane; i < a.slices * a.k; i += 64) {
-      const uint64_t mine = lists[i];
-      if (mine == 0) continue;
-      const int64_t own = i / a.k;
-      int64_t rank = i - own * a.k;
-      for (int64_t l = 0; l < a.slices && rank < a.k; ++l) {
-        if (l == own) continue;
-        const uint64_t* list = lists + l * a.k;
-        int lo = 0, hi = a.k;            // entries that are better
-        while (lo < hi) {
-          const int mid = (lo + hi) / 2;
-          if (list[mid] > mine) lo = mid + 1;
-          else hi = mid;
-        }
-        rank += lo;
+    const int64_t entries = a.slices * a.k;
+    auto put = [&](int rank, uint64_t c) {
+      a.top_ids[row * a.k + rank] = id_of(c);
+      a.top_lp[row * a.k + rank] =
+          (float)(((double)logit_of(c) - s.m) * a.inv_t - log_s);
+    };
+    if (a.slices == 1) {
+      for (int i = lane; i < a.k; i += 64) put(i, lists[i]);
+    } else if (entries <= kHeld) {
+      // what the last of some list is better than cannot be in the top; the
+      // others, about k, count how many are better than they
+      uint64_t bar = 0;
+      for (int64_t l = lane; l < a.slices; l += 64)
+        bar = max(bar, lists[l * a.k + a.k - 1]);
+      bar = wave_reduce(bar, Larger{});
+      int n = 0;
+      for (int first = 0; first < entries; first += 64) {
+        const uint64_t c = first + lane < entries ? lists[first + lane] : 0;
+        const bool kept = c != 0 && c >= bar;
+        const uint64_t all = __ballot(kept);
+        if (kept) held[wave][n + __popcll(all & ((1ull << lane) - 1))] = c;
+        n += __popcll(all);
       }
-      if (rank < a.k) {
-        a.top_ids[row * a.k + rank] = id_of(mine);
-        a.top_lp[row * a.k + rank] =
-            (float)(((double)logit_of(mine) - s.m) * a.inv_t - log_s);
+      wave_fence();
+      for (int i = lane; i < n; i += 64) {
+        const uint64_t mine = held[wave][i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += held[wave][j] > mine;
+        if (rank < a.k) put(rank, mine);
+      }
+    } else {
+      // the place of a candidate: its place in its own list, and how many of
+      // each other list are better
+      for (int64_t i = lane; i < entries; i += 64) {
+        const uint64_t mine = lists[i];
+        if (mine == 0) continue;
+        const int64_t own = i / a.k;
+        int64_t rank = i - own * a.k;
+        for (int64_t l = 0; l < a.slices && rank < a.k; ++l) {
+          if (l == own) continue;
+          const uint64_t* list = lists + l * a.k;
+          int lo = 0, hi = a.k;          // entries that are better
+          while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (list[mid] > mine) lo = mid + 1;
+            else hi = mid;
+          }
+          rank += lo;
+        }
+        if (rank < a.k) put((int)rank, mine);
       }
     }
+    wave_fence();                        // `held` is written again
   }
 }
 
@@ -495,22 +549,22 @@ struct DistillArgs {
   int V, k, per_slice;
   int64_t slices;
   Factor f;
-  double t;
+  double t, inv_t;
   float *loss, *q_out;
   RowStats* stats;
   Sums* part;
 };
 
-// A row's entries, two to a lane of the wave that finishes the row: loaded
-// before the row's sums are known.
+// A row's entries, N to a lane of the wave that finishes the row.
+template <int N>
 struct Entries {
-  int64_t id[2];
-  float lp[2], z[2];       // the teacher's, and the student's logit
+  int64_t id[N];
+  float lp[N], z[N];       // the teacher's, and the student's logit
   template <typename T>
   __device__ __forceinline__ void load(const DistillArgs& a, int64_t row,
                                        const T* logits) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < N; ++e) {
       const int i = (threadIdx.x & 63) + 64 * e;
       id[e] = i < a.k ? a.ids[row * a.k + i] : -1;
       lp[e] = id[e] >= 0 ? a.teacher[row * a.k + i] : -INFINITY;
@@ -520,27 +574,33 @@ struct Entries {
   }
 };
 
-// One wave. `ids`, `shares`: k of each in LDS, for this wave alone.
-template <bool TAIL>
-__device__ void finish_distill(const DistillArgs& a, int64_t row,
-                               const Sums& s, const Entries& t, int64_t* ids,
-                               double* shares) {
+// One wave: the loss of a row. log q is the teacher's own number, less what
+// it is normalised by: no logarithm of an entry is taken.
+template <bool TAIL, int N>
+__device__ __forceinline__ void finish_distill(const DistillArgs& a,
+                                               int64_t row, const Sums& s,
+                                               const Entries<N>& t) {
   const int lane = threadIdx.x & 63;
-  double q[2], rest = 0.0;
+  double q[N], all_q = 0.0, rest = 0.0, off = 0.0;
   if constexpr (TAIL) {
-    q[0] = exp((double)t.lp[0]);
-    q[1] = exp((double)t.lp[1]);
-    const double left = 1.0 - wave_reduce(q[0] + q[1], Add{});
-    rest = left <= 0.0 ? 0.0 : left;
+#pragma unroll
+    for (int e = 0; e < N; ++e) all_q += q[e] = exp((double)t.lp[e]);
+    all_q = wave_reduce(all_q, Add{});
+    rest = 1.0 - all_q <= 0.0 ? 0.0 : 1.0 - all_q;    // NaN stays
   } else {
-    const float top = wave_reduce(MaxNan{}(t.lp[0], t.lp[1]), MaxNan{});
-    const bool none = top == -INFINITY;
-    q[0] = none ? 0.0 : exp((double)t.lp[0] - (double)top);
-    q[1] = none ? 0.0 : exp((double)t.lp[1] - (double)top);
-    const double sum = wave_reduce(q[0] + q[1], Add{});
-    if (sum != 0.0) {
-      q[0] /= sum;
-      q[1] /= sum;
+    float top = t.lp[0];
+    if constexpr (N > 1) top = MaxNan{}(top, t.lp[1]);
+    top = wave_reduce(top, MaxNan{});
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      all_q += q[e] = top == -INFINITY ? 0.0
+                                       : exp((double)t.lp[e] - (double)top);
+    all_q = wave_reduce(all_q, Add{});
+    if (all_q != 0.0) {                  // at least 1, or NaN
+      off = (double)top + log(all_q);
+#pragma unroll
+      for (int e = 0; e < N; ++e) q[e] /= all_q;
+      all_q = 1.0;
     }
   }
   const float m = (float)s.m;
@@ -549,17 +609,18 @@ __device__ void finish_distill(const DistillArgs& a, int64_t row,
   const double sum = 1.0 + others, log_s = log1p(others);
   double total = 0.0;
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
+  for (int e = 0; e < N; ++e)
     if (t.z[e] != t.z[e])                    // no such token, or a NaN
       total = NAN;
     else if (q[e] != 0.0)
-      total += q[e] * (log(q[e]) - (((double)t.z[e] - s.m) / a.t - log_s));
+      total += q[e] * (((double)t.lp[e] - off) -
+                       (((double)t.z[e] - s.m) * a.inv_t - log_s));
   total = wave_reduce(total, Add{});
-  double share = wave_reduce(q[0] + q[1], Add{}), shift = 0.0;
+  double share = all_q, shift = 0.0;
   if (TAIL && rest != 0.0 && outside > 0.0) {
     share += rest;
-    total += rest * (log(rest) - (log(outside) - log_s));
-    shift = rest * sum / outside;
+    shift = rest * sum / outside;        // q_t / p_t
+    total += rest * log(shift);
   }
   if (no_distribution(m)) total = NAN;
   if (lane == 0) a.loss[row] = (float)(total * a.t * a.t);
@@ -567,27 +628,44 @@ __device__ void finish_distill(const DistillArgs& a, int64_t row,
   if (lane == 0)
     a.stats[row] = {m, total != total ? NAN : (float)(1.0 / sum),
                     (float)share, (float)(share - shift)};
-  // an id that is named more than once: each of its entries gets the sum
+  // An id that is named more than once: each of its entries gets the sum. The
+  // absent ones are no id's; of ids past 32 bits the loss is NaN anyway.
+  int id[N];
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (lane + 64 * e < a.k) {
-      ids[lane + 64 * e] = t.id[e];
-      shares[lane + 64 * e] = q[e];
+  for (int e = 0; e < N; ++e)
+    id[e] = t.id[e] < 0 ? -1 - lane - 64 * e : (int)t.id[e];
+  bool twice = false;
+#pragma unroll
+  for (int i = 0; i < 64; ++i) {
+    if (i >= a.k) break;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int one = __builtin_amdgcn_readlane(id[e], i);
+#pragma unroll
+      for (int d = 0; d < N; ++d) twice |= one == id[d] && (d != e || i != lane);
     }
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    if (lane + 64 * e >= a.k) break;
-    double all = 0.0;
-    for (int i = 0; i < a.k; ++i) all += ids[i] == t.id[e] ? shares[i] : 0.0;
-    a.q_out[row * a.k + lane + 64 * e] = (float)all;
   }
+  if (__any(twice)) {
+    double sum_q[N] = {};
+    for (int i = 0; i < 64; ++i)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int one = __shfl(id[e], i);
+        const double share_of_one = __shfl(q[e], i);
+#pragma unroll
+        for (int d = 0; d < N; ++d)
+          if (one == id[d]) sum_q[d] += share_of_one;
+      }
+#pragma unroll
+    for (int e = 0; e < N; ++e) q[e] = sum_q[e];
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (lane + 64 * e < a.k) a.q_out[row * a.k + lane + 64 * e] = (float)q[e];
 }
 
 template <typename T, int NT, int NV, bool TAIL>
-__global__ __launch_bounds__(NT, 4) void distill_slice_kernel(
+__global__ __launch_bounds__(NT, 6) void distill_slice_kernel(
     const T* __restrict__ logits, const DistillArgs a) {
   __shared__ float wave_max[NT / 64];
   __shared__ float sums[NT / 64][6];
@@ -597,17 +675,20 @@ __global__ __launch_bounds__(NT, 4) void distill_slice_kernel(
   for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
     const int64_t row = a.slices == 1 ? w : w / a.slices;
     const int base = (int)(w - row * a.slices) * a.per_slice;
-    const int64_t id = tid < a.k ? a.ids[row * a.k + tid] : -1;
+    const int64_t* ids = a.ids + row * a.k;
+    bool live = false;
+    for (int i = tid; i < a.k; i += NT) live |= ids[i] >= 0;
     if constexpr (TAIL)
       for (int i = tid; i < NT * NV / 4; i += NT) bits[i] = 0;
-    if (!__syncthreads_or(id >= 0)) continue;
+    if (!__syncthreads_or(live)) continue;
     const int len = min(a.per_slice, a.V - base);
     Slice<T, NT, NV> s;
     s.load(logits + row * a.zs + base, len);
     if constexpr (TAIL) {
-      const int64_t at = id - base;
-      if (at >= 0 && at < len) {
-        constexpr int E = kVec<T>;
+      constexpr int E = kVec<T>;
+      for (int i = tid; i < a.k; i += NT) {
+        const int64_t at = ids[i] - base;
+        if (at < 0 || at >= len) continue;
         const int piece = (int)at / E, bit = (int)at % E;
         atomicOr(&bits[piece / 4], 1u << (piece % 4 * 8 + bit));
       }
@@ -628,19 +709,18 @@ __global__ __launch_bounds__(NT, 4) void distill_slice_kernel(
   }
 }
 
-// Four rows to a block, a wave each.
-template <typename T, bool TAIL>
+// Four rows to a block, a wave each; N * 64 entries at most.
+template <typename T, bool TAIL, int N>
 __global__ __launch_bounds__(256) void distill_finish_kernel(
     const T* __restrict__ logits, const DistillArgs a) {
-  __shared__ double shares[4][kMaxTop];
-  __shared__ int64_t named[4][kMaxTop];
-  const int wave = threadIdx.x >> 6;
-  for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < a.rows;
-       row += (int64_t)gridDim.x * 4) {
-    Entries t;
+  const int lane = threadIdx.x & 63;
+  for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+       row < a.rows; row += (int64_t)gridDim.x * 4) {
+    Entries<N> t;
     t.load(a, row, logits + row * a.zs);
-    if (!__any(t.id[0] >= 0 || t.id[1] >= 0)) {
-      const int lane = threadIdx.x & 63;
+    bool live = t.id[0] >= 0;
+    if constexpr (N > 1) live |= t.id[1] >= 0;
+    if (!__any(live)) {
       if (lane == 0) a.loss[row] = 0.f;
       if (a.stats) {
         if (lane == 0) a.stats[row] = {0.f, 0.f, 0.f, 0.f};
@@ -648,8 +728,8 @@ __global__ __launch_bounds__(256) void distill_finish_kernel(
       }
       continue;
     }
-    const Sums s = join_sums(a.part + row * a.slices, a.slices, a.f);
-    finish_distill<TAIL>(a, row, s, t, named[wave], shares[wave]);
+    finish_distill<TAIL, N>(
+        a, row, join_sums(a.part + row * a.slices, a.slices, a.f), t);
   }
 }
 
@@ -810,25 +890,26 @@ Factor exp2_factor(double t) {
 }
 
 // Threads and 16-byte vectors of a slice: the smallest block that holds the
-// row, up to 4096 vectors; longer rows in equal slices.
+// row, up to 4096 vectors; longer rows in equal slices. Where that gives fewer
+// blocks than there are compute units, slices of up to 1024.
 struct Cut {
-  int vectors, per_slice;
-  int64_t slices;
+  int64_t each, slices;      // vectors of a slice, slices of a row
 };
 
-Cut cut_row(int V, int per_vector) {
+Cut cut_row(int64_t rows, int V, int per_vector) {
   const int64_t vecs = (V + per_vector - 1) / per_vector;
-  const int64_t few = (vecs + 4095) / 4096;
+  const int64_t most = rows * ((vecs + 4095) / 4096) < 256 ? 1024 : 4096;
+  const int64_t few = (vecs + most - 1) / most;
   const int64_t each = (vecs + few - 1) / few;
-  const int64_t slices = (vecs + each - 1) / each;     // none of them empty
-  const int vectors = each <= 256 ? 1 : each <= 1024 ? 4 : 8;
-  return {vectors, (int)(each * per_vector), slices};
+  return {each, (vecs + each - 1) / each};             // none of them empty
 }
 
+// top: of how many alternatives; a wave by itself has a floor for 64.
 template <typename F>
-void with_cut(const Cut& c, F f) {
-  if (c.vectors == 1) f(Int<256>{}, Int<1>{});
-  else if (c.vectors == 4) f(Int<256>{}, Int<4>{});
+void with_cut(const Cut& c, int top, F f) {
+  if (c.each <= 256 && top <= 16) f(Int<64>{}, Int<4>{});
+  else if (c.each <= 256) f(Int<256>{}, Int<1>{});
+  else if (c.each <= 1024) f(Int<256>{}, Int<4>{});
   else f(Int<512>{}, Int<8>{});
 }
 
@@ -844,8 +925,8 @@ int per_vector(int type) { return type == kF32 ? 4 : 8; }
 }  // namespace
 
 // Slices of a row, and bytes of the record that each leaves.
-int64_t dear_logit_slices(int type, int V) {
-  return cut_row(V, per_vector(type)).slices;
+int64_t dear_logit_slices(int type, int64_t rows, int V) {
+  return cut_row(rows, V, per_vector(type)).slices;
 }
 int64_t dear_slice_bytes() { return sizeof(Sums); }
 
@@ -854,14 +935,14 @@ int dear_logprobs_fwd(hipStream_t st, int type, const void* logits, int64_t zs,
                       int V, int k, double t, float* logprob, float* entropy,
                       float* top_lp, int64_t* top_ids, void* stats, void* part,
                       void* lists) {
-  const Cut cut = cut_row(V, per_vector(type));
-  const LogprobArgs a = {tokens, zs, ignore, rows, V, k, cut.per_slice,
+  const Cut cut = cut_row(rows, V, per_vector(type));
+  const LogprobArgs a = {tokens, zs, ignore, rows, V, k, (int)(cut.each * per_vector(type)),
                          cut.slices, exp2_factor(t), 1.0 / t, logprob, entropy,
                          top_lp, top_ids, (RowStats*)stats, (Sums*)part,
                          (uint64_t*)lists};
   with_type(type, [&](auto zero) {
     using T = decltype(zero);
-    with_cut(cut, [&](auto nt, auto nv) {
+    with_cut(cut, k, [&](auto nt, auto nv) {
       constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
       const dim3 grid(grid_for(rows * cut.slices)), block(NT);
       if (k)
@@ -907,13 +988,13 @@ int dear_distill_fwd(hipStream_t st, int type, bool tail, const void* logits,
                      int64_t zs, const int64_t* ids, const float* teacher,
                      int64_t rows, int V, int k, double t, float* loss,
                      float* q, void* stats, void* part) {
-  const Cut cut = cut_row(V, per_vector(type));
-  const DistillArgs a = {ids, teacher, zs, rows, V, k, cut.per_slice,
-                         cut.slices, exp2_factor(t), t, loss, q,
+  const Cut cut = cut_row(rows, V, per_vector(type));
+  const DistillArgs a = {ids, teacher, zs, rows, V, k, (int)(cut.each * per_vector(type)),
+                         cut.slices, exp2_factor(t), t, 1.0 / t, loss, q,
                          (RowStats*)stats, (Sums*)part};
   with_type(type, [&](auto zero) {
     using T = decltype(zero);
-    with_cut(cut, [&](auto nt, auto nv) {
+    with_cut(cut, 0, [&](auto nt, auto nv) {
       constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
       const dim3 grid(grid_for(rows * cut.slices)), block(NT);
       if (tail)
@@ -924,12 +1005,13 @@ int dear_distill_fwd(hipStream_t st, int type, bool tail, const void* logits,
                            block, 0, st, (const T*)logits, a);
     });
     const dim3 rest(grid_for((rows + 3) / 4));
-    if (tail)
-      hipLaunchKernelGGL((distill_finish_kernel<T, true>), rest, dim3(256), 0,
-                         st, (const T*)logits, a);
-    else
-      hipLaunchKernelGGL((distill_finish_kernel<T, false>), rest, dim3(256), 0,
-                         st, (const T*)logits, a);
+    auto finish = [&](auto with_tail, auto n) {
+      hipLaunchKernelGGL((distill_finish_kernel<T, decltype(with_tail)::value,
+                                                decltype(n)::value>),
+                         rest, dim3(256), 0, st, (const T*)logits, a);
+    };
+    if (k <= 64) tail ? finish(Int<1>{}, Int<1>{}) : finish(Int<0>{}, Int<1>{});
+    else tail ? finish(Int<1>{}, Int<2>{}) : finish(Int<0>{}, Int<2>{});
   });
   return (int)hipGetLastError();
 }
