@@ -11,6 +11,13 @@
 // The backward reads x and the residual again and adds them again: as many
 // bytes as a stored z would cost, and no rounding of z in between. Sums and
 // statistics are fp32; results are rounded once, to their own type.
+//
+// A row lies in the registers of a group of 16, 64, 256 or 1024 threads, up to
+// 16 elements of each, so that it is read once. Groups go round the rows with
+// their columns' weights, and in the backward their columns' sums of dweight
+// and dbias, in registers as well; each block leaves one record of the sums,
+// and a second kernel adds the records up in a fixed order. Rows over 16384
+// elements are read again for each pass instead (the *_long kernels).
 #include <hip/hip_runtime.h>
 
 #include "lm_common.h"
@@ -19,8 +26,287 @@ namespace {
 
 using namespace dear_lm;
 
-constexpr int kThreads = 256;
 constexpr int kMaxBlocks = 1 << 20;   // a launch holds under 2^32 threads
+constexpr int kPerThread = 16;        // elements of a row in one thread
+constexpr int kRecords = 512;         // of dweight and dbias, at most
+
+// E consecutive elements of type T as they lie in memory.
+template <typename T, int E>
+struct Chunk {
+  static constexpr int kLoads = E / kVec<T>;
+  u32x4 raw[kLoads];
+
+  // elements [i, i + E) of a row of H; what lies behind it is zero
+  __device__ __forceinline__ void load(const T* row, int i, int H) {
+    if (i + E <= H) {
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) raw[q] = load16(row + i + q * kVec<T>);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q) raw[q] = u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (i + j < H) put(raw[j / kVec<T>], j % kVec<T>, row[i + j]);
+    }
+  }
+  __device__ __forceinline__ float at(int j) const {
+    return elem<T>(raw[j / kVec<T>], j % kVec<T>);
+  }
+};
+
+template <typename T, int E>
+__device__ __forceinline__ void store_chunk(T* row, int i, int H,
+                                            const float* v) {
+  if (i + E <= H) {
+#pragma unroll
+    for (int q = 0; q < E / kVec<T>; ++q)
+      store16(row + i + q * kVec<T>, pack<T>(v + q * kVec<T>));
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (i + j < H) row[i + j] = static_cast<T>(v[j]);
+  }
+}
+
+// Sums over a group of G threads, in every one of them. Groups of more than a
+// wave are the whole block, and meet at one barrier: `scratch`, two of a wave,
+// takes turns.
+template <int G>
+struct GroupSum {
+  float (*scratch)[G > 64 ? G / 64 : 1][2];
+  int turn = 0;
+  __device__ __forceinline__ void operator()(float& a, float& b) {
+    auto step = [&](auto o) {
+      a = sum_of(lanes<decltype(o)::value>(a));
+      b = sum_of(lanes<decltype(o)::value>(b));
+    };
+    step(Int<1>{});
+    step(Int<2>{});
+    step(Int<4>{});
+    step(Int<8>{});
+    if constexpr (G >= 64) {
+      step(Int<16>{});
+      step(Int<32>{});
+    }
+    if constexpr (G > 64) {
+      if ((threadIdx.x & 63) == 0) {
+        scratch[turn][threadIdx.x >> 6][0] = a;
+        scratch[turn][threadIdx.x >> 6][1] = b;
+      }
+      __syncthreads();
+      a = b = 0.f;
+#pragma unroll
+      for (int i = 0; i < G / 64; ++i) {
+        a += scratch[turn][i][0];
+        b += scratch[turn][i][1];
+      }
+      turn ^= 1;
+    }
+  }
+  __device__ __forceinline__ float operator()(float a) {
+    float none = 0.f;
+    (*this)(a, none);
+    return a;
+  }
+};
+
+// E elements a chunk: 16 bytes of the narrowest type.
+template <typename TX>
+constexpr int kChunk = kVec<TX>;
+
+template <int NV, int E>
+__device__ __forceinline__ void load_columns(float (&v)[NV * E], const void* p,
+                                             int type, int first, int step,
+                                             int H, float none) {
+#pragma unroll
+  for (int c = 0; c < NV; ++c)
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const int i = first + c * step + j;
+      v[c * E + j] = p && i < H ? load_as_float(p, type, i) : none;
+    }
+}
+
+template <typename TX, typename TR, typename TY, bool RES, int G, int NV>
+__global__ __launch_bounds__(G > 256 ? G : 256, 4) void ln_fwd_kernel(
+    const TX* __restrict__ x, int64_t xs, const TR* __restrict__ r, int64_t rs,
+    const void* __restrict__ w, const void* __restrict__ b, int wtype,
+    TY* __restrict__ y, float* __restrict__ mean_out,
+    float* __restrict__ rstd_out, int64_t rows, int H, float eps) {
+  constexpr int E = kChunk<TX>, NT = G > 256 ? G : 256, N = NV * E;
+  __shared__ float scratch[2][G > 64 ? G / 64 : 1][2];
+  GroupSum<G> group_sum{scratch};
+  const int first = (int)(threadIdx.x % G) * E;
+  float wv[N], bv[N];
+  load_columns<NV, E>(wv, w, wtype, first, G * E, H, 1.f);
+  load_columns<NV, E>(bv, b, wtype, first, G * E, H, 0.f);
+  for (int64_t row = (int64_t)blockIdx.x * (NT / G) + threadIdx.x / G;
+       row < rows; row += (int64_t)gridDim.x * (NT / G)) {
+    Chunk<TX, E> cx[NV];
+    Chunk<TR, E> cr[RES ? NV : 1];
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      cx[c].load(x + row * xs, first + c * G * E, H);
+      if constexpr (RES) cr[c].load(r + row * rs, first + c * G * E, H);
+    }
+    float z[N], s = 0.f;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        float v = cx[c].at(j);
+        if constexpr (RES) v += cr[c].at(j);
+        z[c * E + j] = v;
+        s += v;
+      }
+    // divided, so that the mean of equal elements is the element
+    const float mean = group_sum(s) / (float)H;
+    float q = 0.f;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float d = z[c * E + j] - mean;
+        q += first + c * G * E + j < H ? d * d : 0.f;
+      }
+    const float rstd = 1.0f / sqrtf(group_sum(q) / (float)H + eps);
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        z[c * E + j] = fmaf((z[c * E + j] - mean) * rstd, wv[c * E + j],
+                            bv[c * E + j]);
+      store_chunk<TY, E>(y + row * H, first + c * G * E, H, z + c * E);
+    }
+    if (mean_out && threadIdx.x % G == 0) {
+      mean_out[row] = mean;
+      rstd_out[row] = rstd;
+    }
+  }
+}
+
+template <typename TX, typename TR, typename TY, bool RES, int G, int NV>
+__global__ __launch_bounds__(G > 512 ? G : G > 64 ? 256 : 512, 4)
+void ln_bwd_kernel(
+    const TX* __restrict__ x, int64_t xs, const TR* __restrict__ r, int64_t rs,
+    const TY* __restrict__ dy, int64_t dys, const void* __restrict__ w,
+    int wtype, const float* __restrict__ mean_in,
+    const float* __restrict__ rstd_in, TX* __restrict__ dx,
+    TR* __restrict__ dr, float* __restrict__ records, int64_t rows, int H) {
+  constexpr int E = kChunk<TX>, N = NV * E;
+  constexpr int NT = G > 512 ? G : G > 64 ? 256 : 512;
+  __shared__ float scratch[2][G > 64 ? G / 64 : 1][2];
+  GroupSum<G> group_sum{scratch};
+  const int first = (int)(threadIdx.x % G) * E;
+  float wv[N], aw[N] = {}, ab[N] = {};
+  load_columns<NV, E>(wv, w, wtype, first, G * E, H, 1.f);
+  const float inv_h = 1.0f / (float)H;
+  for (int64_t row = (int64_t)blockIdx.x * (NT / G) + threadIdx.x / G;
+       row < rows; row += (int64_t)gridDim.x * (NT / G)) {
+    Chunk<TX, E> cx[NV];
+    Chunk<TR, E> cr[RES ? NV : 1];
+    Chunk<TY, E> cg[NV];
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      cx[c].load(x + row * xs, first + c * G * E, H);
+      if constexpr (RES) cr[c].load(r + row * rs, first + c * G * E, H);
+      cg[c].load(dy + row * dys, first + c * G * E, H);
+    }
+    const float mean = mean_in[row], rstd = rstd_in[row];
+    float n[N], g[N], sg = 0.f, sgn = 0.f;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int i = c * E + j;
+        float z = cx[c].at(j);
+        if constexpr (RES) z += cr[c].at(j);
+        n[i] = (z - mean) * rstd;
+        const float up = cg[c].at(j);
+        aw[i] = fmaf(up, n[i], aw[i]);
+        ab[i] += up;
+        g[i] = up * wv[i];
+        sg += g[i];
+        sgn = fmaf(g[i], n[i], sgn);
+      }
+    group_sum(sg, sgn);
+    sg *= inv_h;
+    sgn *= inv_h;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int i = c * E + j;
+        g[i] = rstd * (g[i] - sg - n[i] * sgn);
+      }
+      if (dx) store_chunk<TX, E>(dx + row * H, first + c * G * E, H, g + c * E);
+      if constexpr (RES)
+        if (dr)
+          store_chunk<TR, E>(dr + row * H, first + c * G * E, H, g + c * E);
+    }
+  }
+  if (!records) return;
+  // the block's groups, one after the other: a fixed order
+  if constexpr (G < 64) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      aw[i] = sum_of(lanes<32>(sum_of(lanes<16>(aw[i]))));
+      ab[i] = sum_of(lanes<32>(sum_of(lanes<16>(ab[i]))));
+    }
+  }
+  float* record = records + (int64_t)blockIdx.x * 2 * H;
+  if constexpr (G > 64) {
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+      store_chunk<float, E>(record, first + c * G * E, H, aw + c * E);
+      store_chunk<float, E>(record + H, first + c * G * E, H, ab + c * E);
+    }
+  } else {
+    __shared__ float total[2][G * N];
+    const int lane = threadIdx.x & 63;
+    for (int turn = 0; turn < NT / 64; ++turn) {
+      if ((int)threadIdx.x >> 6 == turn && lane < G) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          total[0][i * G + lane] = turn ? total[0][i * G + lane] + aw[i]
+                                        : aw[i];
+          total[1][i * G + lane] = turn ? total[1][i * G + lane] + ab[i]
+                                        : ab[i];
+        }
+      }
+      __syncthreads();
+    }
+    for (int i = threadIdx.x; i < 2 * H; i += NT) {
+      const int col = i < H ? i : i - H;
+      // element j of chunk c of thread t: column c * G * E + t * E + j
+      const int c = col / (G * E), t = col % (G * E) / E, j = col % E;
+      record[i] = total[i >= H][(c * E + j) * G + t];
+    }
+  }
+}
+
+// Adds up the records: 64 columns to a block of 1024, 16 threads to a column.
+__global__ __launch_bounds__(1024) void ln_records_kernel(
+    const float* __restrict__ records, int n, int H, void* __restrict__ dw,
+    void* __restrict__ db, int wtype) {
+  __shared__ float part[16][64];
+  const int lane = threadIdx.x & 63, sub = threadIdx.x >> 6;
+  const int64_t i = (int64_t)blockIdx.x * 64 + lane;
+  float s = 0.f;
+  if (i < 2 * (int64_t)H) {
+#pragma unroll 8
+    for (int k = sub; k < n; k += 16) s += records[(int64_t)k * 2 * H + i];
+  }
+  part[sub][lane] = s;
+  __syncthreads();
+  if (sub != 0 || i >= 2 * (int64_t)H) return;
+  for (int k = 1; k < 16; ++k) s += part[k][lane];
+  void* out = i < H ? dw : db;
+  if (out) store_as(out, wtype, i < H ? i : i - H, s);
+}
+
+// ------------------------------------------------------------- long rows
+constexpr int kLongThreads = 1024;
 
 template <typename TX, typename TR, bool RES>
 __device__ __forceinline__ float load_z(const TX* x, const TR* r, int i) {
@@ -30,27 +316,27 @@ __device__ __forceinline__ float load_z(const TX* x, const TR* r, int i) {
 }
 
 template <typename TX, typename TR, typename TY, bool RES>
-__global__ __launch_bounds__(kThreads) void ln_fwd_kernel(
+__global__ __launch_bounds__(kLongThreads) void ln_fwd_long_kernel(
     const TX* __restrict__ x, int64_t xs, const TR* __restrict__ r, int64_t rs,
     const void* __restrict__ w, const void* __restrict__ b, int wtype,
     TY* __restrict__ y, float* __restrict__ mean_out,
     float* __restrict__ rstd_out, int64_t rows, int H, float eps) {
-  __shared__ float scratch[kThreads / 64];
+  __shared__ float scratch[kLongThreads / 64];
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const TX* xr = x + row * xs;
     const TR* rr = RES ? r + row * rs : nullptr;
     float s = 0.f;
-    for (int i = threadIdx.x; i < H; i += kThreads)
+    for (int i = threadIdx.x; i < H; i += kLongThreads)
       s += load_z<TX, TR, RES>(xr, rr, i);
     const float mean = block_reduce(s, Add{}, scratch) / (float)H;
     float v = 0.f;
-    for (int i = threadIdx.x; i < H; i += kThreads) {
+    for (int i = threadIdx.x; i < H; i += kLongThreads) {
       const float d = load_z<TX, TR, RES>(xr, rr, i) - mean;
       v += d * d;
     }
     const float var = block_reduce(v, Add{}, scratch) / (float)H;
     const float rstd = 1.0f / sqrtf(var + eps);
-    for (int i = threadIdx.x; i < H; i += kThreads) {
+    for (int i = threadIdx.x; i < H; i += kLongThreads) {
       float n = (load_z<TX, TR, RES>(xr, rr, i) - mean) * rstd;
       if (w) n *= load_as_float(w, wtype, i);
       if (b) n += load_as_float(b, wtype, i);
@@ -64,20 +350,20 @@ __global__ __launch_bounds__(kThreads) void ln_fwd_kernel(
 }
 
 template <typename TX, typename TR, typename TY, bool RES>
-__global__ __launch_bounds__(kThreads) void ln_bwd_dx_kernel(
+__global__ __launch_bounds__(kLongThreads) void ln_bwd_long_kernel(
     const TX* __restrict__ x, int64_t xs, const TR* __restrict__ r, int64_t rs,
     const TY* __restrict__ dy, int64_t dys, const void* __restrict__ w,
     int wtype, const float* __restrict__ mean_in,
     const float* __restrict__ rstd_in, TX* __restrict__ dx,
     TR* __restrict__ dr, int64_t rows, int H) {
-  __shared__ float scratch[kThreads / 64];
+  __shared__ float scratch[kLongThreads / 64];
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const TX* xr = x + row * xs;
     const TR* rr = RES ? r + row * rs : nullptr;
     const TY* gr = dy + row * dys;
     const float mean = mean_in[row], rstd = rstd_in[row];
     float sg = 0.f, sgn = 0.f;
-    for (int i = threadIdx.x; i < H; i += kThreads) {
+    for (int i = threadIdx.x; i < H; i += kLongThreads) {
       float g = to_f(gr[i]);
       if (w) g *= load_as_float(w, wtype, i);
       sg += g;
@@ -85,7 +371,7 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_dx_kernel(
     }
     sg = block_reduce(sg, Add{}, scratch) / (float)H;
     sgn = block_reduce(sgn, Add{}, scratch) / (float)H;
-    for (int i = threadIdx.x; i < H; i += kThreads) {
+    for (int i = threadIdx.x; i < H; i += kLongThreads) {
       float g = to_f(gr[i]);
       if (w) g *= load_as_float(w, wtype, i);
       const float n = (load_z<TX, TR, RES>(xr, rr, i) - mean) * rstd;
@@ -96,76 +382,128 @@ __global__ __launch_bounds__(kThreads) void ln_bwd_dx_kernel(
   }
 }
 
-// Column sums of dy * n and of dy over one stripe of rows: part[stripe][2][H].
+// Records of stripes of rows, for long rows.
 template <typename TX, typename TR, typename TY, bool RES>
-__global__ __launch_bounds__(kThreads) void ln_bwd_dw_kernel(
+__global__ __launch_bounds__(256) void ln_dw_long_kernel(
     const TX* __restrict__ x, int64_t xs, const TR* __restrict__ r, int64_t rs,
     const TY* __restrict__ dy, int64_t dys, const float* __restrict__ mean_in,
-    const float* __restrict__ rstd_in, float* __restrict__ part, int64_t rows,
-    int H) {
+    const float* __restrict__ rstd_in, float* __restrict__ records,
+    int64_t rows, int H) {
   __shared__ float sw[4][64], sb[4][64];
   const int lane = threadIdx.x & 63, sub = threadIdx.x >> 6;
-  const int col = blockIdx.y * 64 + lane;
-  float aw = 0.f, ab = 0.f;
-  if (col < H)
-    for (int64_t row = (int64_t)blockIdx.x * 4 + sub; row < rows;
-         row += (int64_t)gridDim.x * 4) {
-      const float g = to_f(dy[row * dys + col]);
-      const float z = load_z<TX, TR, RES>(x + row * xs,
-                                          RES ? r + row * rs : nullptr, col);
-      aw += g * ((z - mean_in[row]) * rstd_in[row]);
-      ab += g;
+  for (int64_t at = (int64_t)blockIdx.y * 64; at < H;
+       at += (int64_t)gridDim.y * 64) {
+    const int col = (int)at + lane;
+    float aw = 0.f, ab = 0.f;
+    if (col < H)
+      for (int64_t row = (int64_t)blockIdx.x * 4 + sub; row < rows;
+           row += (int64_t)gridDim.x * 4) {
+        const float g = to_f(dy[row * dys + col]);
+        const float z = load_z<TX, TR, RES>(x + row * xs,
+                                            RES ? r + row * rs : nullptr, col);
+        aw += g * ((z - mean_in[row]) * rstd_in[row]);
+        ab += g;
+      }
+    sw[sub][lane] = aw;
+    sb[sub][lane] = ab;
+    __syncthreads();
+    if (sub == 0 && col < H) {
+      float* p = records + (int64_t)blockIdx.x * 2 * H;
+      p[col] = (sw[0][lane] + sw[1][lane]) + (sw[2][lane] + sw[3][lane]);
+      p[H + col] = (sb[0][lane] + sb[1][lane]) + (sb[2][lane] + sb[3][lane]);
     }
-  sw[sub][lane] = aw;
-  sb[sub][lane] = ab;
-  __syncthreads();
-  if (sub == 0 && col < H) {
-    float* p = part + (int64_t)blockIdx.x * 2 * H;
-    p[col] = (sw[0][lane] + sw[1][lane]) + (sw[2][lane] + sw[3][lane]);
-    p[H + col] = (sb[0][lane] + sb[1][lane]) + (sb[2][lane] + sb[3][lane]);
+    __syncthreads();
   }
 }
 
-__global__ __launch_bounds__(kThreads) void ln_dw_join_kernel(
-    const float* __restrict__ part, int nparts, int H, void* __restrict__ dw,
-    void* __restrict__ db, int wtype) {
-  const int i = blockIdx.x * kThreads + threadIdx.x;
-  if (i >= 2 * H) return;
-  void* out = i < H ? dw : db;
-  if (!out) return;
-  float s = 0.f;
-  for (int k = 0; k < nparts; ++k) s += part[(int64_t)k * 2 * H + i];
-  store_as(out, wtype, i < H ? i : i - H, s);
+// ------------------------------------------------------------------ launches
+// Threads of a row's group, by its width; 0: too long for registers.
+int group_of(int H, int chunk) {
+  return H <= 16 * chunk ? 16 : H <= 64 * kPerThread ? 64
+         : H <= 256 * kPerThread ? 256 : H <= 1024 * kPerThread ? 1024 : 0;
+}
+
+int64_t at_most(int64_t n, int64_t most) { return n < most ? n : most; }
+
+// f(group, chunks of a thread) for the smallest that hold a row
+template <int E, typename F>
+void with_group(int H, F f) {
+  const int group = group_of(H, E);
+  auto chunks = [&](auto g) {
+    constexpr int G = decltype(g)::value;
+    const int n = (H + G * E - 1) / (G * E);
+    if constexpr (G == 16) f(g, Int<1>{});
+    else if constexpr (E == 8) n <= 1 ? f(g, Int<1>{}) : f(g, Int<2>{});
+    else if (n <= 1) f(g, Int<1>{});
+    else if (n <= 2) f(g, Int<2>{});
+    else if (n <= 3) f(g, Int<3>{});
+    else f(g, Int<4>{});
+  };
+  if (group == 16) chunks(Int<16>{});
+  else if (group == 64) chunks(Int<64>{});
+  else if (group == 256) chunks(Int<256>{});
+  else if (group == 1024) chunks(Int<1024>{});
+}
+
+int64_t bwd_blocks(int64_t rows, int H, int chunk) {
+  const int group = group_of(H, chunk);
+  if (group == 0) return at_most((rows + 31) / 32, 256);
+  const int per_block = group > 64 ? 1 : 512 / group;
+  return at_most((rows + per_block - 1) / per_block, kRecords);
 }
 
 template <typename TX, typename TR, typename TY, bool RES>
 void fwd(hipStream_t st, const void* x, int64_t xs, const void* r, int64_t rs,
          const void* w, const void* b, int wtype, void* y, float* mean,
          float* rstd, int64_t rows, int H, float eps) {
-  const int grid = (int)(rows < kMaxBlocks ? rows : kMaxBlocks);
-  hipLaunchKernelGGL((ln_fwd_kernel<TX, TR, TY, RES>), dim3(grid), dim3(kThreads), 0, st, 
-      (const TX*)x, xs, (const TR*)r, rs, w, b, wtype, (TY*)y, mean, rstd,
-      rows, H, eps);
+  if (group_of(H, kChunk<TX>) == 0) {
+    hipLaunchKernelGGL((ln_fwd_long_kernel<TX, TR, TY, RES>),
+                       dim3(at_most(rows, kMaxBlocks)), dim3(kLongThreads), 0,
+                       st, (const TX*)x, xs, (const TR*)r, rs, w, b, wtype,
+                       (TY*)y, mean, rstd, rows, H, eps);
+    return;
+  }
+  with_group<kChunk<TX>>(H, [&](auto g, auto nv) {
+    constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
+    constexpr int NT = G > 256 ? G : 256;
+    const int64_t blocks = (rows + NT / G - 1) / (NT / G);
+    hipLaunchKernelGGL((ln_fwd_kernel<TX, TR, TY, RES, G, NV>),
+                       dim3(at_most(blocks, 2048)), dim3(NT), 0, st,
+                       (const TX*)x, xs, (const TR*)r, rs, w, b, wtype, (TY*)y,
+                       mean, rstd, rows, H, eps);
+  });
 }
 
 template <typename TX, typename TR, typename TY, bool RES>
 void bwd(hipStream_t st, const void* x, int64_t xs, const void* r, int64_t rs,
          const void* dy, int64_t dys, const void* w, int wtype,
          const float* mean, const float* rstd, void* dx, void* dr, void* dw,
-         void* db, float* part, int nparts, int64_t rows, int H) {
-  if (dx || dr) {
-    const int grid = (int)(rows < kMaxBlocks ? rows : kMaxBlocks);
-    hipLaunchKernelGGL((ln_bwd_dx_kernel<TX, TR, TY, RES>), dim3(grid), dim3(kThreads), 0, st, 
-        (const TX*)x, xs, (const TR*)r, rs, (const TY*)dy, dys, w, wtype, mean,
-        rstd, (TX*)dx, (TR*)dr, rows, H);
+         void* db, float* records, int n, int64_t rows, int H) {
+  if (group_of(H, kChunk<TX>) == 0) {
+    if (dx || dr)
+      hipLaunchKernelGGL((ln_bwd_long_kernel<TX, TR, TY, RES>),
+                         dim3(at_most(rows, kMaxBlocks)), dim3(kLongThreads),
+                         0, st, (const TX*)x, xs, (const TR*)r, rs,
+                         (const TY*)dy, dys, w, wtype, mean, rstd, (TX*)dx,
+                         (TR*)dr, rows, H);
+    if (records)
+      hipLaunchKernelGGL((ln_dw_long_kernel<TX, TR, TY, RES>),
+                         dim3(n, at_most((H + 63) / 64, 65535)), dim3(256), 0,
+                         st, (const TX*)x, xs, (const TR*)r, rs, (const TY*)dy,
+                         dys, mean, rstd, records, rows, H);
+  } else {
+    with_group<kChunk<TX>>(H, [&](auto g, auto nv) {
+      constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
+      constexpr int NT = G > 512 ? G : G > 64 ? 256 : 512;
+      hipLaunchKernelGGL((ln_bwd_kernel<TX, TR, TY, RES, G, NV>), dim3(n),
+                         dim3(NT), 0, st, (const TX*)x, xs, (const TR*)r, rs,
+                         (const TY*)dy, dys, w, wtype, mean, rstd, (TX*)dx,
+                         (TR*)dr, records, rows, H);
+    });
   }
-  if (dw || db) {
-    hipLaunchKernelGGL((ln_bwd_dw_kernel<TX, TR, TY, RES>), dim3(dim3(nparts, (H + 63) / 64)), dim3(kThreads), 0, st, 
-            (const TX*)x, xs, (const TR*)r, rs, (const TY*)dy, dys, mean, rstd,
-            part, rows, H);
-    hipLaunchKernelGGL((ln_dw_join_kernel), dim3((2 * H + kThreads - 1) / kThreads), dim3(kThreads), 0, st, 
-        part, nparts, H, dw, db, wtype);
-  }
+  if (records)
+    hipLaunchKernelGGL(ln_records_kernel, dim3((2 * (int64_t)H + 63) / 64),
+                       dim3(1024), 0, st, records, n, H, dw, db, wtype);
 }
 
 }  // namespace
@@ -184,10 +522,9 @@ void bwd(hipStream_t st, const void* x, int64_t xs, const void* r, int64_t rs,
   } else if (xtype == kBF16) CALL(bf16, float, float, true);                  \
   else CALL(f16, float, float, true)
 
-// Floats of workspace that the backward's column sums need.
-int64_t dear_ln_parts(int64_t rows, int H) {
-  const int64_t stripes = (rows + 31) / 32;
-  return stripes < 256 ? stripes : 256;
+// Blocks of the backward, and records of dweight and dbias (2 H floats each).
+int64_t dear_ln_blocks(int xtype, int64_t rows, int H) {
+  return bwd_blocks(rows, H, xtype == kF32 ? 4 : 8);
 }
 
 int dear_ln_fwd(hipStream_t st, int xtype, int rtype, int wtype, const void* x,
@@ -202,14 +539,15 @@ int dear_ln_fwd(hipStream_t st, int xtype, int rtype, int wtype, const void* x,
   return (int)hipGetLastError();
 }
 
+// records: n times 2 H floats, or null where neither dw nor db is wanted.
 int dear_ln_bwd(hipStream_t st, int xtype, int rtype, int wtype, const void* x,
                 int64_t xs, const void* r, int64_t rs, const void* dy,
                 int64_t dys, const void* w, const float* mean,
                 const float* rstd, void* dx, void* dr, void* dw, void* db,
-                float* part, int nparts, int64_t rows, int H) {
+                float* records, int n, int64_t rows, int H) {
 #define CALL(TX, TR, TY, RES)                                                 \
   bwd<TX, TR, TY, RES>(st, x, xs, r, rs, dy, dys, w, wtype, mean, rstd, dx,   \
-                       dr, dw, db, part, nparts, rows, H)
+                       dr, dw, db, records, n, rows, H)
   LN_DISPATCH(CALL);
 #undef CALL
   return (int)hipGetLastError();

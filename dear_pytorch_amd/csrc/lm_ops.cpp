@@ -7,7 +7,7 @@
 #include <hip/hip_runtime.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
-int64_t dear_ln_parts(int64_t rows, int H);
+int64_t dear_ln_blocks(int, int64_t, int);
 int dear_ln_fwd(hipStream_t, int, int, int, const void*, int64_t, const void*,
                 int64_t, const void*, const void*, void*, float*, float*,
                 int64_t, int, float);
@@ -169,18 +169,17 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
       const Tensor xr = as_rows(x, rows, width);
       const Tensor rr = res.defined() ? as_rows(res, rows, width) : Tensor();
       const Tensor gr = as_rows(up[0], rows, width);
-      int64_t parts = 0;
-      if (want_w || want_b) {
-        parts = dear_ln_parts(rows, (int)width);
-        part = at::empty({parts, 2, width}, stats.options());
-      }
+      const int64_t blocks = dear_ln_blocks(type_code(x, "x"), rows,
+                                            (int)width);
+      if (want_w || want_b)
+        part = at::empty({blocks, 2, width}, stats.options());
       check_launch(dear_ln_bwd(
           stream_of(x), type_code(x, "x"),
           res.defined() ? type_code(res, "residual") : -1,
           affine.defined() ? type_code(affine, "weight") : 0, data(xr),
           xr.stride(0), data(rr), res.defined() ? rr.stride(0) : 0, data(gr),
           gr.stride(0), data(w), fdata(stats), fdata(stats) + rows, data(dx),
-          data(dr), data(dw), data(db), fdata(part), (int)parts, rows,
+          data(dr), data(dw), data(db), fdata(part), (int)blocks, rows,
           (int)width));
     }
     return once({dx, dw, db, same ? dx : dr, Tensor()}, "layer_norm");

@@ -484,6 +484,7 @@ __global__ __launch_bounds__(256) void logprobs_finish_kernel(
         a.stats[row] = {m, bad ? NAN : (float)(1.0 / sum), (float)(h - log_s),
                         0.f};
     }
+    if (a.k == 0) continue;              // there are no lists
     const uint64_t* lists = a.lists + row * a.slices * a.k;
     const int64_t entries = a.slices * a.k;
     auto put = [&](int rank, uint64_t c) {

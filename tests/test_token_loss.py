@@ -517,7 +517,11 @@ def test_refusals_of_temperature_and_teacher():
     (33, 257, 8, 2.0), (6, 1000, 128, 1.0), (5, 4097, 64, 4.0),
     (1, 30528, 8, 1.0), (40, 30522, 5, 1.0), (3, 30528, 128, 1.5),
     (2, 70001, 33, 1.0), (3, 131075, 128, 1.0), (300, 129, 1, 1.0),
-    (2, 600011, 20, 1.0)])
+    (2, 600011, 20, 1.0),
+    # rows of several pieces and no alternatives; more lists than are held at
+    # once; enough rows for the longest pieces
+    (2, 70001, 0, 1.0), (300, 30528, 0, 1.0), (2, 600011, 128, 1.0),
+    (300, 40009, 17, 1.0), (150, 70001, 64, 1.0)])
 def test_gpu_logprobs(R, V, top, T, dtype):
     standard_logprobs(R, V, top, T, dtype, "cuda")
 
