@@ -12,7 +12,7 @@
 // bytes as a stored z would cost, and no rounding of z in between. Sums and
 // statistics are fp32; results are rounded once, to their own type.
 //
-// A row lies in the registers of a group of 16, 64, 256 or 1024 threads, up to
+// A row lies in the registers of a group of 16, 32, 64, 256 or 1024 threads, up to
 // 16 elements of each, so that it is read once. Groups go round the rows with
 // their columns' weights, and in the backward their columns' sums of dweight
 // and dbias, in registers as well; each block leaves one record of the sums,
@@ -28,7 +28,6 @@ using namespace dear_lm;
 
 constexpr int kMaxBlocks = 1 << 20;   // a launch holds under 2^32 threads
 constexpr int kPerThread = 16;        // elements of a row in one thread
-constexpr int kRecords = 512;         // of dweight and dbias, at most
 
 // E consecutive elements of type T as they lie in memory.
 template <typename T, int E>
@@ -84,10 +83,8 @@ struct GroupSum {
     step(Int<2>{});
     step(Int<4>{});
     step(Int<8>{});
-    if constexpr (G >= 64) {
-      step(Int<16>{});
-      step(Int<32>{});
-    }
+    if constexpr (G >= 32) step(Int<16>{});
+    if constexpr (G >= 64) step(Int<32>{});
     if constexpr (G > 64) {
       if ((threadIdx.x & 63) == 0) {
         scratch[turn][threadIdx.x >> 6][0] = a;
@@ -114,17 +111,33 @@ struct GroupSum {
 template <typename TX>
 constexpr int kChunk = kVec<TX>;
 
+// A thread's columns of the weight or bias; `none` where there is neither.
+template <typename T, int NV, int E>
+__device__ __forceinline__ void load_typed(float (&v)[NV * E], const void* p,
+                                           int first, int step, int H) {
+  Chunk<T, E> c[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    c[i].load(static_cast<const T*>(p), first + i * step, H);
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < E; ++j) v[i * E + j] = c[i].at(j);
+}
+
 template <int NV, int E>
 __device__ __forceinline__ void load_columns(float (&v)[NV * E], const void* p,
                                              int type, int first, int step,
                                              int H, float none) {
+  if (!p) {
 #pragma unroll
-  for (int c = 0; c < NV; ++c)
-#pragma unroll
-    for (int j = 0; j < E; ++j) {
-      const int i = first + c * step + j;
-      v[c * E + j] = p && i < H ? load_as_float(p, type, i) : none;
-    }
+    for (int i = 0; i < NV * E; ++i) v[i] = none;
+  } else if (type == kF32) {
+    load_typed<float, NV, E>(v, p, first, step, H);
+  } else if constexpr (E == 8) {
+    if (type == kBF16) load_typed<bf16, NV, E>(v, p, first, step, H);
+    else load_typed<f16, NV, E>(v, p, first, step, H);
+  }
 }
 
 template <typename TX, typename TR, typename TY, bool RES, int G, int NV>
@@ -186,7 +199,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 4) void ln_fwd_kernel(
 }
 
 template <typename TX, typename TR, typename TY, bool RES, int G, int NV>
-__global__ __launch_bounds__(G > 512 ? G : G > 64 ? 256 : 512, 4)
+__global__ __launch_bounds__(G > 512 ? G : G > 64 ? 256 : 512,
+                             G > 512 ? 4 : 2)
 void ln_bwd_kernel(
     const TX* __restrict__ x, int64_t xs, const TR* __restrict__ r, int64_t rs,
     const TY* __restrict__ dy, int64_t dys, const void* __restrict__ w,
@@ -250,8 +264,12 @@ void ln_bwd_kernel(
   if constexpr (G < 64) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      aw[i] = sum_of(lanes<32>(sum_of(lanes<16>(aw[i]))));
-      ab[i] = sum_of(lanes<32>(sum_of(lanes<16>(ab[i]))));
+      if constexpr (G < 32) {
+        aw[i] = sum_of(lanes<16>(aw[i]));
+        ab[i] = sum_of(lanes<16>(ab[i]));
+      }
+      aw[i] = sum_of(lanes<32>(aw[i]));
+      ab[i] = sum_of(lanes<32>(ab[i]));
     }
   }
   float* record = records + (int64_t)blockIdx.x * 2 * H;
@@ -419,8 +437,12 @@ __global__ __launch_bounds__(256) void ln_dw_long_kernel(
 // ------------------------------------------------------------------ launches
 // Threads of a row's group, by its width; 0: too long for registers.
 int group_of(int H, int chunk) {
-  return H <= 16 * chunk ? 16 : H <= 64 * kPerThread ? 64
-         : H <= 256 * kPerThread ? 256 : H <= 1024 * kPerThread ? 1024 : 0;
+  return H <= 16 * chunk           ? 16
+         : H <= 32 * chunk         ? 32
+         : H <= 64 * kPerThread    ? 64
+         : H <= 256 * kPerThread   ? 256
+         : H <= 1024 * kPerThread  ? 1024
+                                   : 0;
 }
 
 int64_t at_most(int64_t n, int64_t most) { return n < most ? n : most; }
@@ -432,7 +454,7 @@ void with_group(int H, F f) {
   auto chunks = [&](auto g) {
     constexpr int G = decltype(g)::value;
     const int n = (H + G * E - 1) / (G * E);
-    if constexpr (G == 16) f(g, Int<1>{});
+    if constexpr (G < 64) f(g, Int<1>{});
     else if constexpr (E == 8) n <= 1 ? f(g, Int<1>{}) : f(g, Int<2>{});
     else if (n <= 1) f(g, Int<1>{});
     else if (n <= 2) f(g, Int<2>{});
@@ -440,6 +462,7 @@ void with_group(int H, F f) {
     else f(g, Int<4>{});
   };
   if (group == 16) chunks(Int<16>{});
+  else if (group == 32) chunks(Int<32>{});
   else if (group == 64) chunks(Int<64>{});
   else if (group == 256) chunks(Int<256>{});
   else if (group == 1024) chunks(Int<1024>{});
@@ -449,7 +472,7 @@ int64_t bwd_blocks(int64_t rows, int H, int chunk) {
   const int group = group_of(H, chunk);
   if (group == 0) return at_most((rows + 31) / 32, 256);
   const int per_block = group > 64 ? 1 : 512 / group;
-  return at_most((rows + per_block - 1) / per_block, kRecords);
+  return at_most((rows + per_block - 1) / per_block, group == 256 ? 512 : 256);
 }
 
 template <typename TX, typename TR, typename TY, bool RES>
