@@ -56,6 +56,13 @@ __device__ __forceinline__ void store16(T* p, u32x4 v) {
   __builtin_memcpy(p, &v, 16);
 }
 
+// Past the caches: for what is too large to be found there again.
+template <typename T>
+__device__ __forceinline__ void stream16(T* p, u32x4 v) {
+  typedef u32x4 __attribute__((aligned(2))) any;
+  __builtin_nontemporal_store(v, reinterpret_cast<any*>(p));
+}
+
 // Element j (known when compiled) of 16 bytes, as fp32.
 template <typename T>
 __device__ __forceinline__ float elem(u32x4 v, int j) {

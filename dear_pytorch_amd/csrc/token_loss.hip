@@ -37,6 +37,7 @@ using namespace dear_lm;
 constexpr int kMaxTop = 128;          // entries of a row
 constexpr int kMaxBlocks = 1 << 20;   // a launch holds under 2^32 threads
 constexpr int kCandidates = 1024;     // of a slice's top, kept for ranking
+constexpr int kPieces = 1024;         // of 16 bytes, with one of them or more
 constexpr double kLn2 = 0.69314718055994530942;
 
 // A key that orders as the logits do: larger is better, NaN above all, both
@@ -122,6 +123,21 @@ struct Slice {
   __device__ __forceinline__ void fresh(int v) {
     asm volatile("" : "+v"(raw[v]));
   }
+  // the elements of `mask` become -inf
+  __device__ __forceinline__ void drop(int v, uint32_t mask) {
+    const u32x4 none = minus_inf<T>();
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      uint32_t bits;
+      if constexpr (E == 4) {
+        bits = mask >> w & 1 ? 0xffffffffu : 0u;
+      } else {
+        bits = (mask >> 2 * w & 1 ? 0xffffu : 0u) |
+               (mask >> 2 * w & 2 ? 0xffff0000u : 0u);
+      }
+      raw[v][w] = (raw[v][w] & ~bits) | (none[w] & bits);
+    }
+  }
   // NaN if the thread holds one
   __device__ __forceinline__ float max() {
     float m = -INFINITY;
@@ -176,13 +192,19 @@ __device__ __noinline__ void bisect_top(const T* z, int len, int base, int k,
   __syncthreads();
 }
 
-// Lanes' values in falling order (bitonic, 21 exchanges).
+// Lanes' values in falling order (bitonic, 21 exchanges). Which lanes keep the
+// larger value is known when compiled, as a mask in scalar registers.
 template <int Size, int O>
 __device__ __forceinline__ float exchange(float v) {
-  const int lane = threadIdx.x & 63;
+  constexpr uint64_t keep = [] {
+    uint64_t m = 0;
+    for (int lane = 0; lane < 64; ++lane)
+      if (((lane & O) == 0) == ((lane & Size) == 0)) m |= 1ull << lane;
+    return m;
+  }();
   const Pair p = lanes<O>(v);
-  const bool larger = ((lane & O) == 0) == ((lane & Size) == 0);
-  v = larger ? fmaxf(p.x, p.y) : fminf(p.x, p.y);
+  v = __builtin_amdgcn_inverse_ballot_w64(keep) ? fmaxf(p.x, p.y)
+                                                : fminf(p.x, p.y);
   if constexpr (O > 1) return exchange<Size, O / 2>(v);
   else return v;
 }
@@ -196,60 +218,71 @@ __device__ __forceinline__ float wave_sort(float v) {
 }
 
 // The k best of a slice into found[0..n), in no order; every thread gets n.
-// k is at most NT.
-// Each of NT / 64 waves has ceil(k / waves) elements that reach the smallest
-// of the waves' such maxima of threads: k elements at least reach it, and
-// about k ln(waves) do if the row is in no order. Only those are collected.
+// k is at most NT. Each of the NT / 64 waves has ceil(k / waves) elements that
+// reach the smallest of the waves' such maxima of threads: k elements at least
+// reach it, and about twice k do if the row is in no order. Two steps collect
+// them: the 16-byte pieces that have one, known by their maxima, and then a
+// thread for each element of those, from memory again.
 template <typename T, int NT, int NV>
-__device__ int slice_top(Slice<T, NT, NV>& s, const T* z, int len,
+__device__ int slice_top(const Slice<T, NT, NV>& s, const T* z, int len,
                          int base, int k, float mine, bool has_nan,
                          uint64_t* found, int* count, float* wave_floor,
                          int* scratch) {
-  constexpr int W = NT / 64;
+  constexpr int W = NT / 64, E = kVec<T>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint16_t* pieces = reinterpret_cast<uint16_t*>(found + kCandidates);
   if (!has_nan) {
     const int each = (k + W - 1) / W;
-    float bar;
-    if (each == 1) {
-      bar = wave_reduce(mine, Max{});
-    } else {
-      bar = __shfl(wave_sort(mine), each - 1);
-    }
+    float bar = each == 1 ? wave_reduce(mine, Max{})
+                          : __shfl(wave_sort(mine), each - 1);
     if (lane == 0) wave_floor[wave] = bar;
-    if (threadIdx.x == 0) *count = 0;
+    if (threadIdx.x < 2) count[threadIdx.x] = 0;
     __syncthreads();
     bar = wave_floor[0];
 #pragma unroll
     for (int i = 1; i < W; ++i) bar = fminf(bar, wave_floor[i]);
-    // a bit for each element of the thread that reaches the bar; then one
-    // place for all of the wave's, and the values from memory again
-    constexpr int E = kVec<T>;
-    static_assert(NV * E <= 64, "a bit for each");
-    uint64_t mask = 0;
+    uint64_t has[NV];
+    int all = 0;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      if (!(s.vmax[v] >= bar)) continue;
-      s.fresh(v);
-      uint32_t bits = 0;
-#pragma unroll
-      for (int j = 0; j < E; ++j) bits |= s.at(v, j) >= bar ? 1u << j : 0u;
-      const int left = len - Slice<T, NT, NV>::first(v);
-      if (left < E) bits &= (1u << max(left, 0)) - 1u;
-      mask |= (uint64_t)bits << v * E;
+      has[v] = __ballot(s.vmax[v] >= bar);
+      all += __popcll(has[v]);
     }
-    const int mine_n = __popcll(mask), before = wave_before(mine_n);
     int at = 0;
-    if (lane == 63) at = atomicAdd(count, before + mine_n);
-    at = __shfl(at, 63) + before;
-    for (; mask != 0 && at < kCandidates; mask &= mask - 1, ++at) {
-      const int b = __ffsll((unsigned long long)mask) - 1;
-      const int i = (b / E * NT + (int)threadIdx.x) * E + b % E;
-      found[at] = candidate(to_f(z[i]), base + i);
+    if (lane == 0 && all) at = atomicAdd(count, all);
+    at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int place = at + __builtin_amdgcn_mbcnt_hi(
+                                 (uint32_t)(has[v] >> 32),
+                                 __builtin_amdgcn_mbcnt_lo((uint32_t)has[v], 0));
+      if (s.vmax[v] >= bar && place < kPieces)
+        pieces[place] = (uint16_t)(v * NT + threadIdx.x);
+      at += __popcll(has[v]);
     }
     __syncthreads();
-    const int n = *count;
-    __syncthreads();
-    if (n <= kCandidates) return n;
+    const int n_pieces = *count;
+    if (n_pieces <= kPieces) {
+      // whole waves go round together
+      for (int first = 0; first < n_pieces * E; first += NT) {
+        const int e = first + (int)threadIdx.x;
+        const int i = e < n_pieces * E ? pieces[e / E] * E + e % E : len;
+        const float x = i < len ? to_f(z[i]) : -INFINITY;
+        const bool kept = i < len && x >= bar;
+        const uint64_t them = __ballot(kept);
+        if (them == 0) continue;
+        int place = 0;
+        if (lane == 0) place = atomicAdd(count + 1, __popcll(them));
+        place = __builtin_amdgcn_readfirstlane(place) +
+                __builtin_amdgcn_mbcnt_hi(
+                    (uint32_t)(them >> 32),
+                    __builtin_amdgcn_mbcnt_lo((uint32_t)them, 0));
+        if (kept && place < kCandidates) found[place] = candidate(x, base + i);
+      }
+      __syncthreads();
+      if (count[1] <= kCandidates) return count[1];
+    }
+    __syncthreads();                     // before `count` is used again
   }
   bisect_top<T, NT>(z, len, base, k, found, count, scratch);
   return k;
@@ -295,31 +328,49 @@ __device__ __forceinline__ Sums slice_sums(Slice<T, NT, NV>& s, B bits,
                                            float (*scratch)[6]) {
   constexpr int W = NT / 64, E = kVec<T>;
   float rest = 0.f, e2 = 0.f, in = 0.f, n = 0.f, n_in = 0.f;
+  auto add = [&](int v) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      const float y = (s.at(v, j) - m) * f.c;
+      const float e = __builtin_amdgcn_exp2f(y);
+      rest += e;
+      if constexpr (ENT) e2 = fmaf(e, fmaxf(y, -256.f), e2);  // 0 for -inf
+    }
+  };
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     s.fresh(v);
     uint32_t named = 0;
     if constexpr (B::kTail) named = bits.named[v * NT + threadIdx.x];
-    if (s.vmax[v] != m && named == 0) {
+    if constexpr (B::kTail) {
+      // named and largest elements are counted here, and then are -inf
+      if (s.vmax[v] == m || named != 0) {
+        uint32_t largest = 0;
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float y = (s.at(v, j) - m) * f.c;
-        const float e = __builtin_amdgcn_exp2f(y);
-        rest += e;
-        if constexpr (ENT) e2 = fmaf(e, fmaxf(y, -256.f), e2);  // 0 for -inf
+        for (int j = 0; j < E; ++j) largest |= s.at(v, j) == m ? 1u << j : 0u;
+        n += (float)__popc(largest & ~named);
+        n_in += (float)__popc(largest & named);
+        for (uint32_t left = named & ~largest; left; left &= left - 1) {
+          float z = 0.f;
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (left >> j & 1 && !(left & ((1u << j) - 1))) z = s.at(v, j);
+          in += __builtin_amdgcn_exp2f((z - m) * f.c);
+        }
+        s.drop(v, named | largest);
       }
+      add(v);
+    } else if (s.vmax[v] != m) {
+      add(v);
     } else {
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const float z = s.at(v, j), y = (z - m) * f.c;
         const float e = __builtin_amdgcn_exp2f(y);
-        const bool inside = B::kTail && (named >> j & 1);
         if (z == m) {
-          if (inside) n_in += 1.f;
-          else n += 1.f;
+          n += 1.f;
         } else {
-          if (inside) in += e;
-          else rest += e;
+          rest += e;
           if constexpr (ENT) e2 = fmaf(e, fmaxf(y, -256.f), e2);
         }
       }
@@ -415,8 +466,8 @@ __global__ __launch_bounds__(NT, 6) void logprobs_slice_kernel(
   __shared__ float wave_max[NT / 64], wave_floor[NT / 64];
   __shared__ float sums[NT / 64][6];
   __shared__ int scratch[NT / 64];
-  __shared__ uint64_t found[TOP ? kCandidates : 1];
-  __shared__ int count;
+  __shared__ uint64_t found[TOP ? kCandidates + kPieces / 4 : 1];
+  __shared__ int count[2];
   const int64_t work = a.rows * a.slices;
   for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
     const int64_t row = a.slices == 1 ? w : w / a.slices;
@@ -435,7 +486,7 @@ __global__ __launch_bounds__(NT, 6) void logprobs_slice_kernel(
     if (threadIdx.x == 0) a.part[w] = r;
     if constexpr (TOP) {
       const int k = min(a.k, len);
-      const int n = slice_top(s, z, len, base, k, mine, m != m, found, &count,
+      const int n = slice_top(s, z, len, base, k, mine, m != m, found, count,
                               wave_floor, scratch);
       uint64_t* list = a.lists + w * a.k;
       ranked<NT>(found, n, k, [&](int rank, uint64_t c) { list[rank] = c; });
@@ -735,48 +786,60 @@ __global__ __launch_bounds__(256) void distill_finish_kernel(
 }
 
 // ----------------------------------------------------------------- backward
-// A block of 256 takes a piece of 256 * kPieces vectors of one row.
+// A block of 256 takes 512 vectors of one row.
 constexpr int kBwdThreads = 256;
-constexpr int kPieces = 4;
+constexpr int kBwdVectors = 2;
 template <typename T>
-constexpr int kBwdTokens = kBwdThreads * kPieces * kVec<T>;
+constexpr int kBwdTokens = kBwdThreads * kBwdVectors * kVec<T>;
 
-template <typename T, typename F>
+// Where a gradient is larger than half of the last-level cache it is written
+// past the caches: 4096 x 30528 fp32, 15 % of the rows labelled, takes 86 us
+// instead of 111; of 75 MB, 24 either way, and there what reads it next may
+// find it in the cache.
+constexpr int64_t kStreamBytes = 128 << 20;
+
+template <bool STREAM, typename T>
+__device__ __forceinline__ void store_vec(T* p, u32x4 v) {
+  if constexpr (STREAM) stream16(p, v);
+  else store16(p, v);
+}
+
+template <bool STREAM, typename T, typename F>
 __device__ __forceinline__ void map_piece(const T* z, T* out, int len, F f) {
   constexpr int E = kVec<T>;
-  u32x4 v[kPieces];
+  u32x4 v[kBwdVectors];
 #pragma unroll
-  for (int p = 0; p < kPieces; ++p) {
+  for (int p = 0; p < kBwdVectors; ++p) {
     const int i = (p * kBwdThreads + (int)threadIdx.x) * E;
     if (i + E <= len) v[p] = load16(z + i);
   }
 #pragma unroll
-  for (int p = 0; p < kPieces; ++p) {
+  for (int p = 0; p < kBwdVectors; ++p) {
     const int i = (p * kBwdThreads + (int)threadIdx.x) * E;
     if (i + E <= len) {
       float r[E];
 #pragma unroll
       for (int j = 0; j < E; ++j) r[j] = f(elem<T>(v[p], j));
-      store16(out + i, pack<T>(r));
+      store_vec<STREAM>(out + i, pack<T>(r));
     } else {
       for (int j = i; j < len; ++j) out[j] = static_cast<T>(f(to_f(z[j])));
     }
   }
 }
 
-template <typename T>
+template <bool STREAM, typename T>
 __device__ __forceinline__ void zero_piece(T* out, int len) {
   constexpr int E = kVec<T>;
 #pragma unroll
-  for (int p = 0; p < kPieces; ++p) {
+  for (int p = 0; p < kBwdVectors; ++p) {
     const int i = (p * kBwdThreads + (int)threadIdx.x) * E;
-    if (i + E <= len) store16(out + i, u32x4{0, 0, 0, 0});
+    if (i + E <= len) store_vec<STREAM>(out + i, u32x4{0, 0, 0, 0});
     else
       for (int j = i; j < len; ++j) out[j] = static_cast<T>(0.f);
   }
 }
 
-template <typename T, bool ENT>
+template <typename T, bool ENT, bool STREAM>
 __global__ __launch_bounds__(kBwdThreads) void logprobs_bwd_kernel(
     const T* __restrict__ logits, int64_t zs,
     const int64_t* __restrict__ tokens, const int64_t* __restrict__ top_ids,
@@ -794,7 +857,7 @@ __global__ __launch_bounds__(kBwdThreads) void logprobs_bwd_kernel(
     T* out = dz + row * V + base;
     const RowStats s = stats[row];
     if (s.inv_s == 0.f) {
-      zero_piece(out, len);
+      zero_piece<STREAM>(out, len);
       continue;
     }
     const int64_t token = d_logprob ? tokens[row] : -1;
@@ -816,7 +879,7 @@ __global__ __launch_bounds__(kBwdThreads) void logprobs_bwd_kernel(
         return e * fmaf(dh, fmaf(fmaxf(y, -1e30f), (float)kLn2, s.a), a);
       return e * a;
     };
-    map_piece(z, out, len, spread);
+    map_piece<STREAM>(z, out, len, spread);
     if (!d_logprob && !d_top) continue;
     // the named tokens of this piece again, with what is theirs; the token
     // itself where it is not one of the top
@@ -843,7 +906,7 @@ __global__ __launch_bounds__(kBwdThreads) void logprobs_bwd_kernel(
   }
 }
 
-template <typename T>
+template <typename T, bool STREAM>
 __global__ __launch_bounds__(kBwdThreads) void distill_bwd_kernel(
     const T* __restrict__ logits, int64_t zs,
     const int64_t* __restrict__ ids, const float* __restrict__ q,
@@ -859,11 +922,11 @@ __global__ __launch_bounds__(kBwdThreads) void distill_bwd_kernel(
     T* out = dz + row * V + base;
     const RowStats s = stats[row];
     if (s.inv_s == 0.f) {
-      zero_piece(out, len);
+      zero_piece<STREAM>(out, len);
       continue;
     }
     const float g = d_loss[row] * t, outside = s.inv_s * s.b * g;
-    map_piece(z, out, len, [&](float v) {
+    map_piece<STREAM>(z, out, len, [&](float v) {
       return __builtin_amdgcn_exp2f((v - s.m) * c) * outside;
     });
     __syncthreads();
@@ -970,17 +1033,16 @@ int dear_logprobs_bwd(hipStream_t st, int type, const void* logits, int64_t zs,
     const int64_t pieces = ((int64_t)V + kBwdTokens<T> - 1) / kBwdTokens<T>;
     const dim3 grid(grid_for(rows * pieces)), block(kBwdThreads);
     const float c = exp2_factor(t).c, inv_t = (float)(1.0 / t);
-    const RowStats* s = (const RowStats*)stats;
-    if (d_entropy)
-      hipLaunchKernelGGL((logprobs_bwd_kernel<T, true>), grid, block, 0, st,
-                         (const T*)logits, zs, tokens, top_ids, s, d_logprob,
-                         d_entropy, d_top, (T*)dz, rows, V, pieces, k, c,
-                         inv_t);
-    else
-      hipLaunchKernelGGL((logprobs_bwd_kernel<T, false>), grid, block, 0, st,
-                         (const T*)logits, zs, tokens, top_ids, s, d_logprob,
-                         d_entropy, d_top, (T*)dz, rows, V, pieces, k, c,
-                         inv_t);
+    auto launch = [&](auto ent, auto stream) {
+      hipLaunchKernelGGL((logprobs_bwd_kernel<T, decltype(ent)::value,
+                                              decltype(stream)::value>),
+                         grid, block, 0, st, (const T*)logits, zs, tokens,
+                         top_ids, (const RowStats*)stats, d_logprob, d_entropy,
+                         d_top, (T*)dz, rows, V, pieces, k, c, inv_t);
+    };
+    const bool stream = rows * V * (int64_t)sizeof(T) > kStreamBytes;
+    if (d_entropy) stream ? launch(Int<1>{}, Int<1>{}) : launch(Int<1>{}, Int<0>{});
+    else stream ? launch(Int<0>{}, Int<1>{}) : launch(Int<0>{}, Int<0>{});
   });
   return (int)hipGetLastError();
 }
@@ -1024,10 +1086,15 @@ int dear_distill_bwd(hipStream_t st, int type, const void* logits, int64_t zs,
   with_type(type, [&](auto zero) {
     using T = decltype(zero);
     const int64_t pieces = ((int64_t)V + kBwdTokens<T> - 1) / kBwdTokens<T>;
-    hipLaunchKernelGGL((distill_bwd_kernel<T>), dim3(grid_for(rows * pieces)),
-                       dim3(kBwdThreads), 0, st, (const T*)logits, zs, ids, q,
-                       (const RowStats*)stats, d_loss, (T*)dz, rows, V, pieces,
-                       k, exp2_factor(t).c, (float)t);
+    auto launch = [&](auto stream) {
+      hipLaunchKernelGGL((distill_bwd_kernel<T, decltype(stream)::value>),
+                         dim3(grid_for(rows * pieces)), dim3(kBwdThreads), 0,
+                         st, (const T*)logits, zs, ids, q,
+                         (const RowStats*)stats, d_loss, (T*)dz, rows, V,
+                         pieces, k, exp2_factor(t).c, (float)t);
+    };
+    rows * V * (int64_t)sizeof(T) > kStreamBytes ? launch(Int<1>{})
+                                                 : launch(Int<0>{});
   });
   return (int)hipGetLastError();
 }
