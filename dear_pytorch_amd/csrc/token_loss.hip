@@ -435,13 +435,18 @@ __device__ __forceinline__ Sums join_sums(const Sums* part, int64_t ns,
       r.in += g * (p.n_in + p.in);
     }
   }
-  for (int o = 32; o > 0; o >>= 1) {
+  for (int o = 1; o < 64 && o < ns; o <<= 1) {    // the lanes with a record
     r.n += __shfl_xor(r.n, o);
     r.rest += __shfl_xor(r.rest, o);
     r.e2 += __shfl_xor(r.e2, o);
     r.n_in += __shfl_xor(r.n_in, o);
     r.in += __shfl_xor(r.in, o);
   }
+  r.n = __shfl(r.n, 0);
+  r.rest = __shfl(r.rest, 0);
+  r.e2 = __shfl(r.e2, 0);
+  r.n_in = __shfl(r.n_in, 0);
+  r.in = __shfl(r.in, 0);
   return r;
 }
 
@@ -546,12 +551,17 @@ __global__ __launch_bounds__(256) void logprobs_finish_kernel(
     if (a.slices == 1) {
       for (int i = lane; i < a.k; i += 64) put(i, lists[i]);
     } else if (entries <= kHeld) {
-      // what the last of some list is better than cannot be in the top; the
-      // others, about k, count how many are better than they
-      uint64_t bar = 0;
-      for (int64_t l = lane; l < a.slices; l += 64)
-        bar = max(bar, lists[l * a.k + a.k - 1]);
-      bar = wave_reduce(bar, Larger{});
+      // no better than the last of some list: not in the top. And k of them at
+      // least are as good as the worst of the lists' ceil(k / slices)-th. The
+      // others, little more than k, count how many are better than they
+      const int64_t deep = (a.k + a.slices - 1) / a.slices;
+      uint64_t last = 0, worst = ~0ull;
+      for (int64_t l = lane; l < a.slices; l += 64) {
+        last = max(last, lists[l * a.k + a.k - 1]);
+        worst = min(worst, lists[l * a.k + deep - 1]);
+      }
+      const uint64_t bar = max(wave_reduce(last, Larger{}),
+                               ~wave_reduce(~worst, Larger{}));
       int n = 0;
       for (int first = 0; first < entries; first += 64) {
         const uint64_t c = first + lane < entries ? lists[first + lane] : 0;
@@ -561,11 +571,22 @@ __global__ __launch_bounds__(256) void logprobs_finish_kernel(
         n += __popcll(all);
       }
       wave_fence();
-      for (int i = lane; i < n; i += 64) {
-        const uint64_t mine = held[wave][i];
+      for (int i = 0; i < n; i += 64) {
+        const uint64_t mine = i + lane < n ? held[wave][i + lane] : 0;
         int rank = 0;
-        for (int j = 0; j < n; ++j) rank += held[wave][j] > mine;
-        if (rank < a.k) put(rank, mine);
+        for (int first = 0; first < n; first += 64) {
+          // 64 of them in the lanes, one after the other to all
+          const uint64_t one = first + lane < n ? held[wave][first + lane] : 0;
+          const int many = min(64, n - first);
+          for (int j = 0; j < many; ++j) {
+            const uint64_t c =
+                (uint64_t)(uint32_t)__builtin_amdgcn_readlane(
+                    (int)(one >> 32), j) << 32 |
+                (uint32_t)__builtin_amdgcn_readlane((int)one, j);
+            rank += c > mine;
+          }
+        }
+        if (mine != 0 && rank < a.k) put(rank, mine);
       }
     } else {
       // the place of a candidate: its place in its own list, and how many of
