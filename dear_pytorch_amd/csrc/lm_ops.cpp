@@ -15,7 +15,8 @@ int dear_ln_bwd(hipStream_t, int, int, int, const void*, int64_t, const void*,
                 int64_t, const void*, int64_t, const void*, const float*,
                 const float*, void*, void*, void*, void*, float*, int, int64_t,
                 int);
-int64_t dear_logit_slices(int, int64_t, int);
+int64_t dear_logprobs_slices(int, int64_t, int, int);
+int64_t dear_distill_slices(int, int64_t, int);
 int64_t dear_slice_bytes();
 int dear_logprobs_fwd(hipStream_t, int, const void*, int64_t, const int64_t*,
                       int64_t, int64_t, int, int, double, float*, float*,
@@ -247,10 +248,8 @@ void check_logits(const Tensor& t, const char* name) {
 }
 
 // What the slices of rows leave for the kernel that joins them
-Tensor slice_records(const Tensor& logits, const LogitRows& z) {
-  const int64_t n = dear_logit_slices(type_code(logits, "logits"), z.rows,
-                                      z.width);
-  return at::empty({z.rows * n, dear_slice_bytes()},
+Tensor slice_records(const Tensor& logits, int64_t rows, int64_t slices) {
+  return at::empty({rows * slices, dear_slice_bytes()},
                    logits.options().dtype(at::kByte));
 }
 
@@ -275,7 +274,9 @@ variable_list logprobs_forward(const Tensor& logits, const Tensor& tokens,
   if (z.rows) {
     const Tensor tok = tokens.defined() ? tokens.contiguous() : Tensor();
     const int type = type_code(logits, "logits");
-    const Tensor part = slice_records(logits, z);
+    const Tensor part = slice_records(
+        logits, z.rows,
+        dear_logprobs_slices(type, z.rows, z.width, (int)top));
     Tensor lists;
     if (top)
       lists = at::empty({part.size(0), top}, logits.options().dtype(at::kLong));
@@ -380,9 +381,11 @@ Tensor distill_forward(const Tensor& logits, const Tensor& ids,
   if (z.rows) {
     const Tensor idc = ids.contiguous();
     const Tensor tc = teacher.to(at::kFloat).contiguous();
-    const Tensor part = slice_records(logits, z);
+    const int type = type_code(logits, "logits");
+    const Tensor part = slice_records(
+        logits, z.rows, dear_distill_slices(type, z.rows, z.width));
     check_launch(dear_distill_fwd(
-        stream_of(logits), type_code(logits, "logits"), tail, data(z.t),
+        stream_of(logits), type, tail, data(z.t),
         z.t.dim() == 2 ? z.t.stride(0) : 0, idata(idc), fdata(tc), z.rows,
         z.width, (int)k, t, fdata(loss), q ? fdata(*q) : nullptr,
         stats ? data(*stats) : nullptr, data(part)));

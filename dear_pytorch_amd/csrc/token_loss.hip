@@ -974,27 +974,34 @@ Factor exp2_factor(double t) {
   return {(float)exact, exact};
 }
 
-// Threads and 16-byte vectors of a slice: the smallest block that holds the
-// row, up to 4096 vectors; longer rows in equal slices. Where that gives fewer
-// blocks than there are compute units, slices of up to 1024.
+// Slices of a row, of up to `most` 16-byte vectors; of up to 1024 where that
+// would give fewer blocks than there are compute units. Smaller slices overlap
+// their phases better, larger ones leave fewer lists to make and join. Of 4096
+// and 2048 vectors, us: 614 of 4096 rows of 30528 fp32, no top, 28.8 and 25.0;
+// 4096 rows of 30528 bf16 with a top of 32 75.8 and 79.9, of 128 122 and 198;
+// distillation with a tail, 4096 rows of 30528 bf16, 66.9 and 69.0. One row of
+// 30528 fp32 with a top of 8: 12.3 of 4096, 11.6 of 1024, 12.9 of 512 vectors.
 struct Cut {
   int64_t each, slices;      // vectors of a slice, slices of a row
 };
+constexpr int kLargeSlice = 4096, kSmallSlice = 2048;
 
-Cut cut_row(int64_t rows, int V, int per_vector) {
+Cut cut_row(int64_t rows, int V, int per_vector, int64_t most) {
   const int64_t vecs = (V + per_vector - 1) / per_vector;
-  const int64_t most = rows * ((vecs + 4095) / 4096) < 256 ? 1024 : 4096;
+  if (rows * ((vecs + most - 1) / most) < 256) most = 1024;
   const int64_t few = (vecs + most - 1) / most;
   const int64_t each = (vecs + few - 1) / few;
   return {each, (vecs + each - 1) / each};             // none of them empty
 }
 
-// top: of how many alternatives; a wave by itself has a floor for 64.
+// The smallest block that holds a slice; top: of how many alternatives. A wave
+// by itself has a floor for no more than 64, and ranks them slowly.
 template <typename F>
 void with_cut(const Cut& c, int top, F f) {
   if (c.each <= 256 && top <= 16) f(Int<64>{}, Int<4>{});
   else if (c.each <= 256) f(Int<256>{}, Int<1>{});
   else if (c.each <= 1024) f(Int<256>{}, Int<4>{});
+  else if (c.each <= 2048) f(Int<256>{}, Int<8>{});
   else f(Int<512>{}, Int<8>{});
 }
 
@@ -1010,8 +1017,12 @@ int per_vector(int type) { return type == kF32 ? 4 : 8; }
 }  // namespace
 
 // Slices of a row, and bytes of the record that each leaves.
-int64_t dear_logit_slices(int type, int64_t rows, int V) {
-  return cut_row(rows, V, per_vector(type)).slices;
+int64_t dear_logprobs_slices(int type, int64_t rows, int V, int k) {
+  return cut_row(rows, V, per_vector(type), k ? kLargeSlice : kSmallSlice)
+      .slices;
+}
+int64_t dear_distill_slices(int type, int64_t rows, int V) {
+  return cut_row(rows, V, per_vector(type), kLargeSlice).slices;
 }
 int64_t dear_slice_bytes() { return sizeof(Sums); }
 
@@ -1020,9 +1031,11 @@ int dear_logprobs_fwd(hipStream_t st, int type, const void* logits, int64_t zs,
                       int V, int k, double t, float* logprob, float* entropy,
                       float* top_lp, int64_t* top_ids, void* stats, void* part,
                       void* lists) {
-  const Cut cut = cut_row(rows, V, per_vector(type));
-  const LogprobArgs a = {tokens, zs, ignore, rows, V, k, (int)(cut.each * per_vector(type)),
-                         cut.slices, exp2_factor(t), 1.0 / t, logprob, entropy,
+  const Cut cut = cut_row(rows, V, per_vector(type),
+                          k ? kLargeSlice : kSmallSlice);
+  const LogprobArgs a = {tokens, zs, ignore, rows, V, k,
+                         (int)(cut.each * per_vector(type)), cut.slices,
+                         exp2_factor(t), 1.0 / t, logprob, entropy,
                          top_lp, top_ids, (RowStats*)stats, (Sums*)part,
                          (uint64_t*)lists};
   with_type(type, [&](auto zero) {
@@ -1072,9 +1085,10 @@ int dear_distill_fwd(hipStream_t st, int type, bool tail, const void* logits,
                      int64_t zs, const int64_t* ids, const float* teacher,
                      int64_t rows, int V, int k, double t, float* loss,
                      float* q, void* stats, void* part) {
-  const Cut cut = cut_row(rows, V, per_vector(type));
-  const DistillArgs a = {ids, teacher, zs, rows, V, k, (int)(cut.each * per_vector(type)),
-                         cut.slices, exp2_factor(t), t, 1.0 / t, loss, q,
+  const Cut cut = cut_row(rows, V, per_vector(type), kLargeSlice);
+  const DistillArgs a = {ids, teacher, zs, rows, V, k,
+                         (int)(cut.each * per_vector(type)), cut.slices,
+                         exp2_factor(t), t, 1.0 / t, loss, q,
                          (RowStats*)stats, (Sums*)part};
   with_type(type, [&](auto zero) {
     using T = decltype(zero);
