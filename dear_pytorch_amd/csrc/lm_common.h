@@ -196,6 +196,33 @@ __device__ __forceinline__ float wave_reduce(float v, Op op) {
   p = lanes<32>(v);
   return op(p.x, p.y);
 }
+// The same exchange of both halves of a double, and the wave's sum of two.
+template <int O>
+__device__ __forceinline__ double sum_pair(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const Pair lo = lanes<O>(__uint_as_float((uint32_t)u));
+  const Pair hi = lanes<O>(__uint_as_float((uint32_t)(u >> 32)));
+  auto join = [](float h, float l) {
+    return __builtin_bit_cast(double, (uint64_t)__float_as_uint(h) << 32 |
+                                          __float_as_uint(l));
+  };
+  return join(hi.x, lo.x) + join(hi.y, lo.y);
+}
+__device__ __forceinline__ void wave_sum(double& a, double& b) {
+  a = sum_pair<1>(a);
+  b = sum_pair<1>(b);
+  a = sum_pair<2>(a);
+  b = sum_pair<2>(b);
+  a = sum_pair<4>(a);
+  b = sum_pair<4>(b);
+  a = sum_pair<8>(a);
+  b = sum_pair<8>(b);
+  a = sum_pair<16>(a);
+  b = sum_pair<16>(b);
+  a = sum_pair<32>(a);
+  b = sum_pair<32>(b);
+}
+
 template <typename A, typename Op>
 __device__ __forceinline__ A wave_reduce(A v, Op op) {
 #pragma unroll

@@ -635,47 +635,45 @@ struct Entries {
 };
 
 // One wave: the loss of a row. log q is the teacher's own number, less what
-// it is normalised by: no logarithm of an entry is taken.
+// it is normalised by: no logarithm of an entry is taken. Without a tail, with
+// u_k = exp(lp_k - top) and U = sum u, q_k = u_k / U and
+//   sum q_k (log q_k - l_k) = sum u_k ((lp_k - top) - l_k) / U - log U.
 template <bool TAIL, int N>
 __device__ __forceinline__ void finish_distill(const DistillArgs& a,
                                                int64_t row, const Sums& s,
                                                const Entries<N>& t) {
   const int lane = threadIdx.x & 63;
-  double q[N], all_q = 0.0, rest = 0.0, off = 0.0;
-  if constexpr (TAIL) {
-#pragma unroll
-    for (int e = 0; e < N; ++e) all_q += q[e] = exp((double)t.lp[e]);
-    all_q = wave_reduce(all_q, Add{});
-    rest = 1.0 - all_q <= 0.0 ? 0.0 : 1.0 - all_q;    // NaN stays
-  } else {
-    float top = t.lp[0];
+  float top = 0.f;
+  if constexpr (!TAIL) {
+    top = t.lp[0];
     if constexpr (N > 1) top = MaxNan{}(top, t.lp[1]);
     top = wave_reduce(top, MaxNan{});
-#pragma unroll
-    for (int e = 0; e < N; ++e)
-      all_q += q[e] = top == -INFINITY ? 0.0
-                                       : exp((double)t.lp[e] - (double)top);
-    all_q = wave_reduce(all_q, Add{});
-    if (all_q != 0.0) {                  // at least 1, or NaN
-      off = (double)top + log(all_q);
-#pragma unroll
-      for (int e = 0; e < N; ++e) q[e] /= all_q;
-      all_q = 1.0;
-    }
   }
   const float m = (float)s.m;
   const double outside = s.n + s.rest;
   const double others = (s.rest + s.in) + ((s.n + s.n_in) - 1.0);
   const double sum = 1.0 + others, log_s = log1p(others);
-  double total = 0.0;
+  double q[N], all_q = 0.0, total = 0.0, rest = 0.0;
 #pragma unroll
-  for (int e = 0; e < N; ++e)
+  for (int e = 0; e < N; ++e) {
+    const double lq = (double)t.lp[e] - (double)top;
+    q[e] = top == -INFINITY ? 0.0 : exp(lq);
+    all_q += q[e];
     if (t.z[e] != t.z[e])                    // no such token, or a NaN
       total = NAN;
     else if (q[e] != 0.0)
-      total += q[e] * (((double)t.lp[e] - off) -
-                       (((double)t.z[e] - s.m) * a.inv_t - log_s));
-  total = wave_reduce(total, Add{});
+      total += q[e] * (lq - (((double)t.z[e] - s.m) * a.inv_t - log_s));
+  }
+  wave_sum(all_q, total);
+  if constexpr (TAIL) {
+    rest = 1.0 - all_q <= 0.0 ? 0.0 : 1.0 - all_q;    // NaN stays
+  } else if (all_q != 0.0) {             // at least 1, or NaN
+    const double by = 1.0 / all_q;
+    total = total * by - log(all_q);
+#pragma unroll
+    for (int e = 0; e < N; ++e) q[e] *= by;
+    all_q = 1.0;
+  }
   double share = all_q, shift = 0.0;
   if (TAIL && rest != 0.0 && outside > 0.0) {
     share += rest;
@@ -995,9 +993,10 @@ Factor exp2_factor(double t) {
 // would give fewer blocks than there are compute units. Smaller slices overlap
 // their phases better, larger ones leave fewer lists to make and join. Of 4096
 // and 2048 vectors, us: 614 of 4096 rows of 30528 fp32, no top, 28.8 and 25.0;
-// 4096 rows of 30528 bf16 with a top of 32 75.8 and 79.9, of 128 122 and 198;
-// distillation with a tail, 4096 rows of 30528 bf16, 66.9 and 69.0. One row of
-// 30528 fp32 with a top of 8: 12.3 of 4096, 11.6 of 1024, 12.9 of 512 vectors.
+// 4096 rows of 30528 bf16 with a top of 32 76.0 and 79.5, of 128 123 and 197;
+// distillation of the same with a tail 59.5 and 57.8, without 52.3 and 50.6.
+// One row of 30528 fp32 with a top of 8: 12.3 of 4096, 11.6 of 1024, 12.9 of
+// 512 vectors.
 struct Cut {
   int64_t each, slices;      // vectors of a slice, slices of a row
 };
@@ -1039,7 +1038,7 @@ int64_t dear_logprobs_slices(int type, int64_t rows, int V, int k) {
       .slices;
 }
 int64_t dear_distill_slices(int type, int64_t rows, int V) {
-  return cut_row(rows, V, per_vector(type), kLargeSlice).slices;
+  return cut_row(rows, V, per_vector(type), kSmallSlice).slices;
 }
 int64_t dear_slice_bytes() { return sizeof(Sums); }
 
@@ -1102,7 +1101,7 @@ int dear_distill_fwd(hipStream_t st, int type, bool tail, const void* logits,
                      int64_t zs, const int64_t* ids, const float* teacher,
                      int64_t rows, int V, int k, double t, float* loss,
                      float* q, void* stats, void* part) {
-  const Cut cut = cut_row(rows, V, per_vector(type), kLargeSlice);
+  const Cut cut = cut_row(rows, V, per_vector(type), kSmallSlice);
   const DistillArgs a = {ids, teacher, zs, rows, V, k,
                          (int)(cut.each * per_vector(type)), cut.slices,
                          exp2_factor(t), t, 1.0 / t, loss, q,
