@@ -154,41 +154,55 @@ struct Slice {
   }
 };
 
-// The lists of a slice's top, by bisection in memory: the largest key that at
-// least k elements reach, then, among the elements equal to it, the lowest
-// ids. For rows whose order the quick way cannot use: NaN, or very many equal
-// elements. 31 + 32 passes over the slice.
+// A slice's top by counting in memory, for rows whose order the quick way
+// cannot use: NaN, or very many equal elements (a mask that leaves less than k
+// tokens). bar: k elements at least reach it, or NaN where nothing is known.
+// Where less than k are above it, these and the first ones equal to it are the
+// top: the row is passed over once, and again to where the last one is found.
+// Else the largest key that k elements reach comes first, in 32 more passes.
 template <typename T, int NT>
-__device__ __noinline__ void bisect_top(const T* z, int len, int base, int k,
-                           uint64_t* found, int* count, int* scratch) {
-  uint32_t key = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t want = key | (1u << bit);
+__device__ __noinline__ void count_top(const T* z, int len, int base, int k,
+                                       float bar, uint64_t* found, int* count,
+                                       int* scratch) {
+  constexpr int W = NT / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto reach = [&](uint32_t key) {       // elements with this key or a larger
     int n = 0;
     for (int i = threadIdx.x; i < len; i += NT)
-      n += order_key(to_f(z[i])) >= want;
-    if (block_reduce(n, Add{}, scratch) >= k) key = want;
-  }
-  int above = 0;
-  for (int i = threadIdx.x; i < len; i += NT)
-    above += order_key(to_f(z[i])) > key;
-  const int need = k - block_reduce(above, Add{}, scratch);
-  int low = 0, high = len - 1;           // smallest index that has `need`
-  while (low < high) {
-    const int mid = low + (high - low) / 2;
-    int n = 0;
-    for (int i = threadIdx.x; i <= mid; i += NT)
-      n += order_key(to_f(z[i])) == key;
-    if (block_reduce(n, Add{}, scratch) >= need) high = mid;
-    else low = mid + 1;
+      n += order_key(to_f(z[i])) >= key;
+    return block_reduce(n, Add{}, scratch);
+  };
+  uint32_t key = order_key(bar);
+  int above = key == 0xffffffffu ? k : reach(key + 1);
+  if (above >= k) {
+    key = 0;
+    for (int bit = 31; bit >= 0; --bit)
+      if (reach(key | (1u << bit)) >= k) key |= 1u << bit;
+    above = key == 0xffffffffu ? 0 : reach(key + 1);
   }
   if (threadIdx.x == 0) *count = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < len; i += NT) {
+  for (int i = threadIdx.x; i < len && above > 0; i += NT) {
     const float v = to_f(z[i]);
-    const uint32_t u = order_key(v);
-    if (u > key || (u == key && i <= low))
-      found[atomicAdd(count, 1)] = candidate(v, base + i);
+    if (order_key(v) > key) found[atomicAdd(count, 1)] = candidate(v, base + i);
+  }
+  // found[above, k): those equal to it, in the order of their ids
+  for (int first = 0, at = above; first < len && at < k; first += NT) {
+    const int i = first + (int)threadIdx.x;
+    const float v = i < len ? to_f(z[i]) : 0.f;
+    const bool equal = i < len && order_key(v) == key;
+    const uint64_t them = __ballot(equal);
+    __syncthreads();                     // `scratch` has been read
+    if (lane == 0) scratch[wave] = __popcll(them);
+    __syncthreads();
+    int place = at;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      if (w < wave) place += scratch[w];
+      at += scratch[w];
+    }
+    place += __popcll(them & ((1ull << lane) - 1));
+    if (equal && place < k) found[place] = candidate(v, base + i);
   }
   __syncthreads();
 }
@@ -232,10 +246,11 @@ __device__ int slice_top(const Slice<T, NT, NV>& s, const T* z, int len,
   constexpr int W = NT / 64, E = kVec<T>;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint16_t* pieces = reinterpret_cast<uint16_t*>(found + kCandidates);
+  float bar = NAN;
   if (!has_nan) {
     const int each = (k + W - 1) / W;
-    float bar = each == 1 ? wave_reduce(mine, Max{})
-                          : __shfl(wave_sort(mine), each - 1);
+    bar = each == 1 ? wave_reduce(mine, Max{})
+                    : __shfl(wave_sort(mine), each - 1);
     if (lane == 0) wave_floor[wave] = bar;
     if (threadIdx.x < 2) count[threadIdx.x] = 0;
     __syncthreads();
@@ -285,7 +300,7 @@ __device__ int slice_top(const Slice<T, NT, NV>& s, const T* z, int len,
     }
     __syncthreads();                     // before `count` is used again
   }
-  bisect_top<T, NT>(z, len, base, k, found, count, scratch);
+  count_top<T, NT>(z, len, base, k, bar, found, count, scratch);
   return k;
 }
 
