@@ -12,12 +12,12 @@
 // bytes as a stored z would cost, and no rounding of z in between. Sums and
 // statistics are fp32; results are rounded once, to their own type.
 //
-// A row lies in the registers of a group of 16, 32, 64, 256 or 1024 threads, up to
-// 16 elements of each, so that it is read once. Groups go round the rows with
-// their columns' weights, and in the backward their columns' sums of dweight
-// and dbias, in registers as well; each block leaves one record of the sums,
-// and a second kernel adds the records up in a fixed order. Rows over 16384
-// elements are read again for each pass instead (the *_long kernels).
+// A row lies in the registers of a group of 16, 32, 64, 256 or 1024 threads,
+// up to 16 elements of each, so that it is read once. Groups go round the rows
+// with their columns' weights, and in the backward their columns' sums of
+// dweight and dbias, in registers as well; each block leaves one record of the
+// sums, and a second kernel adds the records up in a fixed order. Rows over
+// 16384 elements are read again for each pass instead (the *_long kernels).
 #include <hip/hip_runtime.h>
 
 #include "lm_common.h"

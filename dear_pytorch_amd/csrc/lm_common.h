@@ -168,16 +168,11 @@ __device__ __forceinline__ void wave_fence() {
 
 __device__ __forceinline__ float sum_of(Pair p) { return p.x + p.y; }
 
-// The sum over the lanes below this one.
-__device__ __forceinline__ int wave_before(int v) {
-  const int lane = threadIdx.x & 63;
-  int s = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int w = __shfl_up(s, o);
-    if (lane >= o) s += w;
-  }
-  return s - v;
+// How many lanes below this one have their bit in a ballot.
+__device__ __forceinline__ int lanes_before(uint64_t ballot) {
+  return __builtin_amdgcn_mbcnt_hi(
+      (uint32_t)(ballot >> 32),
+      __builtin_amdgcn_mbcnt_lo((uint32_t)ballot, 0));
 }
 
 // Reductions over the wave, in every lane.

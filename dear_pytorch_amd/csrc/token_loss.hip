@@ -87,7 +87,6 @@ __device__ __forceinline__ bool no_distribution(float m) {
 template <typename T, int NT, int NV>
 struct Slice {
   static constexpr int E = kVec<T>;
-  static constexpr int kTokens = NT * NV * E;
   u32x4 raw[NV];
   float vmax[NV];
 
@@ -146,9 +145,9 @@ struct Slice {
     for (int v = 0; v < NV; ++v) {
       float a = at(v, 0);
 #pragma unroll
-      for (int j = 1; j < E; ++j) a = __builtin_elementwise_maximum(a, at(v, j));
+      for (int j = 1; j < E; ++j) a = MaxNan{}(a, at(v, j));
       vmax[v] = a;
-      m = __builtin_elementwise_maximum(m, a);
+      m = MaxNan{}(m, a);
     }
     return m;
   }
@@ -201,7 +200,7 @@ __device__ __noinline__ void count_top(const T* z, int len, int base, int k,
       if (w < wave) place += scratch[w];
       at += scratch[w];
     }
-    place += __popcll(them & ((1ull << lane) - 1));
+    place += lanes_before(them);
     if (equal && place < k) found[place] = candidate(v, base + i);
   }
   __syncthreads();
@@ -269,9 +268,7 @@ __device__ int slice_top(const Slice<T, NT, NV>& s, const T* z, int len,
     at = __builtin_amdgcn_readfirstlane(at);
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      const int place = at + __builtin_amdgcn_mbcnt_hi(
-                                 (uint32_t)(has[v] >> 32),
-                                 __builtin_amdgcn_mbcnt_lo((uint32_t)has[v], 0));
+      const int place = at + lanes_before(has[v]);
       if (s.vmax[v] >= bar && place < kPieces)
         pieces[place] = (uint16_t)(v * NT + threadIdx.x);
       at += __popcll(has[v]);
@@ -289,10 +286,7 @@ __device__ int slice_top(const Slice<T, NT, NV>& s, const T* z, int len,
         if (them == 0) continue;
         int place = 0;
         if (lane == 0) place = atomicAdd(count + 1, __popcll(them));
-        place = __builtin_amdgcn_readfirstlane(place) +
-                __builtin_amdgcn_mbcnt_hi(
-                    (uint32_t)(them >> 32),
-                    __builtin_amdgcn_mbcnt_lo((uint32_t)them, 0));
+        place = __builtin_amdgcn_readfirstlane(place) + lanes_before(them);
         if (kept && place < kCandidates) found[place] = candidate(x, base + i);
       }
       __syncthreads();
@@ -452,7 +446,7 @@ __device__ __forceinline__ Sums join_sums(const Sums* part, int64_t ns,
   return r;
 }
 
-// --------------------------------------------------- log probabilities, forward
+// ------------------------------------------------- log probabilities, forward
 struct LogprobArgs {
   const int64_t* tokens;
   int64_t zs, ignore, rows;
@@ -569,7 +563,7 @@ __global__ __launch_bounds__(256) void logprobs_finish_kernel(
         const uint64_t c = first + lane < entries ? lists[first + lane] : 0;
         const bool kept = c != 0 && c >= bar;
         const uint64_t all = __ballot(kept);
-        if (kept) held[wave][n + __popcll(all & ((1ull << lane) - 1))] = c;
+        if (kept) held[wave][n + lanes_before(all)] = c;
         n += __popcll(all);
       }
       wave_fence();
@@ -715,7 +709,8 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a,
     for (int e = 0; e < N; ++e) {
       const int one = __builtin_amdgcn_readlane(id[e], i);
 #pragma unroll
-      for (int d = 0; d < N; ++d) twice |= one == id[d] && (d != e || i != lane);
+      for (int d = 0; d < N; ++d)
+        twice |= one == id[d] && (d != e || i != lane);
     }
   }
   if (__any(twice)) {
@@ -1025,15 +1020,27 @@ Cut cut_row(int64_t rows, int V, int per_vector, int64_t most) {
   return {each, (vecs + each - 1) / each};             // none of them empty
 }
 
-// The smallest block that holds a slice; top: of how many alternatives. A wave
-// by itself has a floor for no more than 64, and ranks them slowly.
-template <typename F>
-void with_cut(const Cut& c, int top, F f) {
-  if (c.each <= 256 && top <= 16) f(Int<64>{}, Int<4>{});
-  else if (c.each <= 256) f(Int<256>{}, Int<1>{});
-  else if (c.each <= 1024) f(Int<256>{}, Int<4>{});
-  else if (c.each <= 2048) f(Int<256>{}, Int<8>{});
-  else f(Int<512>{}, Int<8>{});
+// The smallest block that holds a slice. k: of how many alternatives, 0 of
+// none. A wave by itself has a floor for no more than 64 of them, and ranks
+// them slowly.
+template <bool TOP, typename F>
+void with_cut(const Cut& c, int k, F f) {
+  if (c.each <= 256 && k <= 16) {
+    f(Int<64>{}, Int<4>{});
+    return;
+  }
+  if constexpr (TOP) {
+    if (c.each <= 256) {
+      f(Int<256>{}, Int<1>{});
+      return;
+    }
+    if (c.each > kSmallSlice) {
+      f(Int<512>{}, Int<8>{});
+      return;
+    }
+  }
+  if (c.each <= 1024) f(Int<256>{}, Int<4>{});
+  else f(Int<256>{}, Int<8>{});
 }
 
 template <typename F>
@@ -1071,16 +1078,19 @@ int dear_logprobs_fwd(hipStream_t st, int type, const void* logits, int64_t zs,
                          (uint64_t*)lists};
   with_type(type, [&](auto zero) {
     using T = decltype(zero);
-    with_cut(cut, k, [&](auto nt, auto nv) {
+    const dim3 grid(grid_for(rows * cut.slices));
+    auto launch = [&](auto nt, auto nv, auto top) {
       constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
-      const dim3 grid(grid_for(rows * cut.slices)), block(NT);
-      if (k)
-        hipLaunchKernelGGL((logprobs_slice_kernel<T, NT, NV, true>), grid,
-                           block, 0, st, (const T*)logits, a);
-      else
-        hipLaunchKernelGGL((logprobs_slice_kernel<T, NT, NV, false>), grid,
-                           block, 0, st, (const T*)logits, a);
-    });
+      hipLaunchKernelGGL(
+          (logprobs_slice_kernel<T, NT, NV, decltype(top)::value>), grid,
+          dim3(NT), 0, st, (const T*)logits, a);
+    };
+    if (k)
+      with_cut<true>(cut, k,
+                     [&](auto nt, auto nv) { launch(nt, nv, Int<1>{}); });
+    else
+      with_cut<false>(cut, 0,
+                      [&](auto nt, auto nv) { launch(nt, nv, Int<0>{}); });
     hipLaunchKernelGGL((logprobs_finish_kernel<T>),
                        dim3(grid_for((rows + 3) / 4)), dim3(256), 0, st,
                        (const T*)logits, a);
@@ -1106,8 +1116,10 @@ int dear_logprobs_bwd(hipStream_t st, int type, const void* logits, int64_t zs,
                          d_top, (T*)dz, rows, V, pieces, k, c, inv_t);
     };
     const bool stream = rows * V * (int64_t)sizeof(T) > kStreamBytes;
-    if (d_entropy) stream ? launch(Int<1>{}, Int<1>{}) : launch(Int<1>{}, Int<0>{});
-    else stream ? launch(Int<0>{}, Int<1>{}) : launch(Int<0>{}, Int<0>{});
+    auto with_ent = [&](auto ent) {
+      stream ? launch(ent, Int<1>{}) : launch(ent, Int<0>{});
+    };
+    d_entropy ? with_ent(Int<1>{}) : with_ent(Int<0>{});
   });
   return (int)hipGetLastError();
 }
@@ -1123,7 +1135,7 @@ int dear_distill_fwd(hipStream_t st, int type, bool tail, const void* logits,
                          (RowStats*)stats, (Sums*)part};
   with_type(type, [&](auto zero) {
     using T = decltype(zero);
-    with_cut(cut, 0, [&](auto nt, auto nv) {
+    with_cut<false>(cut, 0, [&](auto nt, auto nv) {
       constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
       const dim3 grid(grid_for(rows * cut.slices)), block(NT);
       if (tail)

@@ -18,7 +18,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from ..ops.fused_ln import FusedLayerNorm
-from ..ops.token_loss import (TokenLogProbs, token_logprobs,
+from ..ops.token_loss import (MAX_TOP, TokenLogProbs, token_logprobs,
                               topk_distill_loss)
 
 __all__ = ["BertConfig", "BertForPreTraining", "BertPretrainingCriterion",
@@ -202,8 +202,9 @@ class BertDistillationCriterion(BertPretrainingCriterion):
         super().__init__(vocab_size, fused=True)
         if not 0.0 <= weight <= 1.0:
             raise ValueError(f"weight must be 0 to 1, got {weight}")
-        if not 1 <= top <= vocab_size:
-            raise ValueError(f"top must be 1 to the vocabulary, got {top}")
+        if not 1 <= top <= min(MAX_TOP, vocab_size):
+            raise ValueError(f"top must be 1 to {MAX_TOP} and at most the "
+                             f"vocabulary, got {top}")
         self.top, self.temperature = top, temperature
         self.weight, self.tail = weight, tail
 

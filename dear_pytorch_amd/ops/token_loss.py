@@ -134,10 +134,10 @@ def topk_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor,
 
         temperature^2 * KL(teacher || softmax(logits / temperature))
 
-    logits [..., V]; top_ids int64 [..., K] and top_logprobs [..., K], K of 1
-    to MAX_TOP. Entries with a negative id are absent; a row with no entry has
-    loss 0 and gradient 0 and is not looked at. An id that is named twice
-    counts with the sum of its shares.
+    logits [..., V]; top_ids int64 [..., K] and top_logprobs [..., K] (float32
+    or 16-bit), K of 1 to MAX_TOP. Entries with a negative id are absent; a row
+    with no entry has loss 0 and gradient 0 and is not looked at. An id that is
+    named twice counts with the sum of its shares.
 
     top_logprobs are the teacher's log probabilities at this temperature.
     tail=False: the teacher is their softmax over the named tokens, so that

@@ -108,7 +108,8 @@ def test_distillation_criterion_follows_its_formula():
     want.backward()
     assert abs(loss - want) < 1e-12 * want
     assert off(grads, {n: p.grad for n, p in model.named_parameters()}) < 1e-11
-    for bad in (dict(weight=1.5), dict(top=0), dict(top=VOCAB + 1)):
+    for bad in (dict(weight=1.5), dict(top=0), dict(top=129),
+                dict(top=VOCAB + 1)):
         with pytest.raises(ValueError):
             models.BertDistillationCriterion(VOCAB, **bad)
 

@@ -509,6 +509,11 @@ def test_refusals_of_temperature_and_teacher():
         topk_distill_loss(z, ids, lp.requires_grad_(True))
 
 
+def test_most_entries():
+    kernels = pytest.importorskip("dear_pytorch_amd._kernels")
+    assert kernels.max_top == MAX_TOP
+
+
 # ------------------------------------------------------------------ on a GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
