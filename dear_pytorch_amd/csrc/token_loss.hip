@@ -66,10 +66,10 @@ struct RowStats {
   float m, inv_s, a, b;
 };
 
-// log2(e) / T and what fp32 leaves of it.
+// log2(e) / T, what fp32 leaves of it, and ln 2 times what that loses.
 struct Factor {
   float c;
-  double exact;
+  double exact, lost;
 };
 
 // The sums of a slice or of a row, relative to its maximum m: n elements are
@@ -81,6 +81,31 @@ struct Sums {
 
 __device__ __forceinline__ bool no_distribution(float m) {
   return !(fabsf(m) < INFINITY);
+}
+
+// log(1 + x), x >= 0, in few registers: with 1 + x = 2^k (1 + f), 1 + f from
+// sqrt(1/2) to sqrt(2), and r = f / (2 + f), |r| < 0.1716,
+//   log(1 + f) = 2 (r + r^3/3 + r^5/5 + ...)
+// up to r^17/17, relatively to 2^-50; f is x itself where k = 0.
+__device__ __forceinline__ double log_1p(double x) {
+  double f = x;
+  float k = 0.f;
+  if (x > 0.41421356237309504880) {
+    const double y = 1.0 + x;
+    int e = __builtin_amdgcn_frexp_exp(y);
+    f = __builtin_amdgcn_frexp_mant(y);
+    if (f < 0.70710678118654752440) {
+      f += f;
+      --e;
+    }
+    f -= 1.0;
+    k = (float)e;
+  }
+  const double r = f / (2.0 + f), r2 = r * r;
+  double p = 1.0 / 17.0;
+#pragma unroll
+  for (int i = 15; i > 0; i -= 2) p = fma(p, r2, 1.0 / i);
+  return fma((double)k, kLn2, 2.0 * r * p);
 }
 
 // ------------------------------------------------------- a slice in registers
@@ -397,7 +422,7 @@ __device__ __forceinline__ Sums slice_sums(Slice<T, NT, NV>& s, float m,
       }
     }
     // exp2(y c_exact / c) of every element, to first order (2^-25 squared)
-    if constexpr (ENT) r.rest += (f.exact / (double)f.c - 1.0) * kLn2 * r.e2;
+    if constexpr (ENT) r.rest += f.lost * r.e2;
   }
   r.m = m;
   return r;
@@ -461,19 +486,67 @@ struct LogprobArgs {
   uint64_t* lists;           // [rows][slices][k], best first, 0: no such one
 };
 
-template <typename T, int NT, int NV, bool TOP>
-__global__ __launch_bounds__(NT, 6) void logprobs_slice_kernel(
+// A row that is not looked at, by `threads` threads.
+__device__ __forceinline__ void leave_out(const LogprobArgs& a, int64_t row,
+                                          int thread, int threads) {
+  if (thread == 0) {
+    a.logprob[row] = 0.f;
+    a.entropy[row] = 0.f;
+    if (a.stats) a.stats[row] = {0.f, 0.f, 0.f, 0.f};
+  }
+  for (int i = thread; i < a.k; i += threads) {
+    a.top_lp[row * a.k + i] = -INFINITY;
+    a.top_ids[row * a.k + i] = -1;
+  }
+}
+
+// The numbers of a row from its sums, written by the `first` thread; log s to
+// all.
+template <typename T>
+__device__ __forceinline__ double finish_row(const LogprobArgs& a, int64_t row,
+                                             const T* z, const Sums& s,
+                                             bool first) {
+  const float m = (float)s.m;
+  const bool bad = no_distribution(m);
+  const double others = s.rest + (s.n - 1.0);
+  const double log_s = bad ? NAN : log_1p(others);
+  if (!first) return log_s;
+  const double inv = 1.0 / (1.0 + others), h = log_s - kLn2 * s.e2 * inv;
+  a.entropy[row] = (float)h;
+  if (a.tokens) {
+    const int64_t token = a.tokens[row];
+    const float at = token >= 0 && token < a.V ? to_f(z[token]) : NAN;
+    a.logprob[row] = (float)(((double)at - s.m) * a.inv_t - log_s);
+  }
+  if (a.stats)
+    a.stats[row] = {m, bad ? NAN : (float)inv, (float)(h - log_s), 0.f};
+  return log_s;
+}
+
+__device__ __forceinline__ void put_top(const LogprobArgs& a, int64_t place,
+                                        uint64_t c, double m, double log_s) {
+  a.top_ids[place] = id_of(c);
+  a.top_lp[place] = (float)(((double)logit_of(c) - m) * a.inv_t - log_s);
+}
+
+// WHOLE: a slice is a whole row, and is finished here.
+template <typename T, int NT, int NV, bool TOP, bool WHOLE>
+__global__ __launch_bounds__(NT, WHOLE ? 4 : 6) void logprobs_slice_kernel(
     const T* __restrict__ logits, const LogprobArgs a) {
   __shared__ float wave_max[NT / 64], wave_floor[NT / 64];
   __shared__ float sums[NT / 64][6];
   __shared__ int scratch[NT / 64];
   __shared__ uint64_t found[TOP ? kCandidates + kPieces / 4 : 1];
   __shared__ int count[2];
+  __shared__ double row_log_s;
   const int64_t work = a.rows * a.slices;
   for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
-    const int64_t row = a.slices == 1 ? w : w / a.slices;
+    const int64_t row = WHOLE || a.slices == 1 ? w : w / a.slices;
     const int base = (int)(w - row * a.slices) * a.per_slice;
-    if (a.tokens && a.tokens[row] == a.ignore) continue;
+    if (a.tokens && a.tokens[row] == a.ignore) {
+      if constexpr (WHOLE) leave_out(a, row, threadIdx.x, NT);
+      continue;
+    }
     const T* z = logits + row * a.zs + base;
     const int len = min(a.per_slice, a.V - base);
     Slice<T, NT, NV> s;
@@ -484,14 +557,26 @@ __global__ __launch_bounds__(NT, 6) void logprobs_slice_kernel(
     if (!no_distribution(m))
       r = slice_sums<T, NT, NV, true, false>(s, m, a.f, 0, 0.f, 0.f, sums);
     r.m = m;
-    if (threadIdx.x == 0) a.part[w] = r;
+    if constexpr (!WHOLE) {
+      if (threadIdx.x == 0) a.part[w] = r;
+    } else if (threadIdx.x < 64) {       // while the others begin with the top
+      const double log_s = finish_row(a, row, z, r, threadIdx.x == 0);
+      if (threadIdx.x == 0) row_log_s = log_s;
+    }
     if constexpr (TOP) {
       const int k = min(a.k, len);
       const int n = slice_top(s, z, len, base, k, mine, m != m, found, count,
                               wave_floor, scratch);
-      uint64_t* list = a.lists + w * a.k;
-      ranked<NT>(found, n, k, [&](int rank, uint64_t c) { list[rank] = c; });
-      for (int i = k + threadIdx.x; i < a.k; i += NT) list[i] = 0;
+      if constexpr (WHOLE) {             // k is a.k
+        const double log_s = row_log_s;
+        ranked<NT>(found, n, k, [&](int rank, uint64_t c) {
+          put_top(a, row * a.k + rank, c, m, log_s);
+        });
+      } else {
+        uint64_t* list = a.lists + w * a.k;
+        ranked<NT>(found, n, k, [&](int rank, uint64_t c) { list[rank] = c; });
+        for (int i = k + threadIdx.x; i < a.k; i += NT) list[i] = 0;
+      }
     }
     __syncthreads();                     // before the arrays are used again
   }
@@ -506,43 +591,18 @@ __global__ __launch_bounds__(256) void logprobs_finish_kernel(
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < a.rows;
        row += (int64_t)gridDim.x * 4) {
-    const int64_t token = a.tokens ? a.tokens[row] : -1;
-    if (a.tokens && token == a.ignore) {
-      if (lane == 0) {
-        a.logprob[row] = 0.f;
-        a.entropy[row] = 0.f;
-        if (a.stats) a.stats[row] = {0.f, 0.f, 0.f, 0.f};
-      }
-      for (int i = lane; i < a.k; i += 64) {
-        a.top_lp[row * a.k + i] = -INFINITY;
-        a.top_ids[row * a.k + i] = -1;
-      }
+    if (a.tokens && a.tokens[row] == a.ignore) {
+      leave_out(a, row, lane, 64);
       continue;
     }
-    const float at = token >= 0 && token < a.V
-                         ? to_f(logits[row * a.zs + token])
-                         : NAN;
     const Sums s = join_sums(a.part + row * a.slices, a.slices, a.f);
-    const float m = (float)s.m;
-    const bool bad = no_distribution(m);
-    const double others = s.rest + (s.n - 1.0), sum = 1.0 + others;
-    const double log_s = bad ? NAN : log1p(others);
-    const double h = log_s - kLn2 * s.e2 / sum;
-    if (lane == 0) {
-      a.entropy[row] = (float)h;
-      if (a.tokens)
-        a.logprob[row] = (float)(((double)at - s.m) * a.inv_t - log_s);
-      if (a.stats)
-        a.stats[row] = {m, bad ? NAN : (float)(1.0 / sum), (float)(h - log_s),
-                        0.f};
-    }
+    const double log_s =
+        finish_row(a, row, logits + row * a.zs, s, lane == 0);
     if (a.k == 0) continue;              // there are no lists
     const uint64_t* lists = a.lists + row * a.slices * a.k;
     const int64_t entries = a.slices * a.k;
     auto put = [&](int rank, uint64_t c) {
-      a.top_ids[row * a.k + rank] = id_of(c);
-      a.top_lp[row * a.k + rank] =
-          (float)(((double)logit_of(c) - s.m) * a.inv_t - log_s);
+      put_top(a, row * a.k + rank, c, s.m, log_s);
     };
     if (a.slices == 1) {
       for (int i = lane; i < a.k; i += 64) put(i, lists[i]);
@@ -661,7 +721,7 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a,
   const float m = (float)s.m;
   const double outside = s.n + s.rest;
   const double others = (s.rest + s.in) + ((s.n + s.n_in) - 1.0);
-  const double sum = 1.0 + others, log_s = log1p(others);
+  const double sum = 1.0 + others, log_s = log_1p(others);
   double q[N], all_q = 0.0, total = 0.0, rest = 0.0;
 #pragma unroll
   for (int e = 0; e < N; ++e) {
@@ -996,7 +1056,7 @@ int grid_for(int64_t work) {
 // log2(e) / T: exp(t) is exp2 of the distance times this
 Factor exp2_factor(double t) {
   const double exact = 1.4426950408889634074 / t;
-  return {(float)exact, exact};
+  return {(float)exact, exact, (exact / (double)(float)exact - 1.0) * kLn2};
 }
 
 // Slices of a row, of up to `most` 16-byte vectors; of up to 1024 where that
@@ -1020,14 +1080,40 @@ Cut cut_row(int64_t rows, int V, int per_vector, int64_t most) {
   return {each, (vecs + each - 1) / each};             // none of them empty
 }
 
+// Log probabilities of few rows: a block to each row if it can hold that, which
+// then needs no second kernel. A row of 30528 fp32 with a top of 8, us: 11.5 in
+// slices, 9.0 whole; 64 such rows 13.2 and 10.8.
+constexpr int kWhole = 8192;
+Cut cut_logprobs(int type, int64_t rows, int V, int k) {
+  const int E = type == kF32 ? 4 : 8;
+  const int64_t vecs = ((int64_t)V + E - 1) / E;
+  if (rows < 256 && vecs <= kWhole) return {vecs, 1};
+  return cut_row(rows, V, E, k ? kLargeSlice : kSmallSlice);
+}
+
+// Whether rows that are one slice are finished in their block: where all of
+// them run at once (4 waves on each SIMD) this saves a launch, and with more
+// the larger kernel's registers cost more than that. Us, apart and together:
+// 4096 x 1000 fp32, top 4, 14.7 and 10.7; 300 x 30528 bf16, top 32, 16.6 and
+// 15.1; 4096 x 30528 bf16, top 32, 76 and 90.
+bool finish_there(const Cut& c, int64_t rows, int threads) {
+  return c.slices == 1 && rows * threads <= 256 * 16 * 64;
+}
+
 // The smallest block that holds a slice. k: of how many alternatives, 0 of
 // none. A wave by itself has a floor for no more than 64 of them, and ranks
 // them slowly.
-template <bool TOP, typename F>
+template <bool TOP, int MOST, typename F>
 void with_cut(const Cut& c, int k, F f) {
   if (c.each <= 256 && k <= 16) {
     f(Int<64>{}, Int<4>{});
     return;
+  }
+  if constexpr (MOST > kLargeSlice) {
+    if (c.each > kLargeSlice) {
+      f(Int<1024>{}, Int<8>{});
+      return;
+    }
   }
   if constexpr (TOP) {
     if (c.each <= 256) {
@@ -1056,8 +1142,7 @@ int per_vector(int type) { return type == kF32 ? 4 : 8; }
 
 // Slices of a row, and bytes of the record that each leaves.
 int64_t dear_logprobs_slices(int type, int64_t rows, int V, int k) {
-  return cut_row(rows, V, per_vector(type), k ? kLargeSlice : kSmallSlice)
-      .slices;
+  return cut_logprobs(type, rows, V, k).slices;
 }
 int64_t dear_distill_slices(int type, int64_t rows, int V) {
   return cut_row(rows, V, per_vector(type), kSmallSlice).slices;
@@ -1069,8 +1154,7 @@ int dear_logprobs_fwd(hipStream_t st, int type, const void* logits, int64_t zs,
                       int V, int k, double t, float* logprob, float* entropy,
                       float* top_lp, int64_t* top_ids, void* stats, void* part,
                       void* lists) {
-  const Cut cut = cut_row(rows, V, per_vector(type),
-                          k ? kLargeSlice : kSmallSlice);
+  const Cut cut = cut_logprobs(type, rows, V, k);
   const LogprobArgs a = {tokens, zs, ignore, rows, V, k,
                          (int)(cut.each * per_vector(type)), cut.slices,
                          exp2_factor(t), 1.0 / t, logprob, entropy,
@@ -1078,22 +1162,31 @@ int dear_logprobs_fwd(hipStream_t st, int type, const void* logits, int64_t zs,
                          (uint64_t*)lists};
   with_type(type, [&](auto zero) {
     using T = decltype(zero);
-    const dim3 grid(grid_for(rows * cut.slices));
-    auto launch = [&](auto nt, auto nv, auto top) {
+    auto launch = [&](auto nt, auto nv, auto top, auto whole) {
       constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
       hipLaunchKernelGGL(
-          (logprobs_slice_kernel<T, NT, NV, decltype(top)::value>), grid,
-          dim3(NT), 0, st, (const T*)logits, a);
+          (logprobs_slice_kernel<T, NT, NV, decltype(top)::value,
+                                 decltype(whole)::value>),
+          dim3(grid_for(rows * cut.slices)), dim3(NT), 0, st,
+          (const T*)logits, a);
+    };
+    auto run = [&](auto nt, auto nv, auto top) {
+      if (finish_there(cut, rows, decltype(nt)::value)) {
+        launch(nt, nv, top, Int<1>{});
+        return;
+      }
+      // rows that need a block of 1024 are always finished there
+      if constexpr (decltype(nt)::value < 1024) launch(nt, nv, top, Int<0>{});
+      hipLaunchKernelGGL((logprobs_finish_kernel<T>),
+                         dim3(grid_for((rows + 3) / 4)), dim3(256), 0, st,
+                         (const T*)logits, a);
     };
     if (k)
-      with_cut<true>(cut, k,
-                     [&](auto nt, auto nv) { launch(nt, nv, Int<1>{}); });
+      with_cut<true, kWhole>(
+          cut, k, [&](auto nt, auto nv) { run(nt, nv, Int<1>{}); });
     else
-      with_cut<false>(cut, 0,
-                      [&](auto nt, auto nv) { launch(nt, nv, Int<0>{}); });
-    hipLaunchKernelGGL((logprobs_finish_kernel<T>),
-                       dim3(grid_for((rows + 3) / 4)), dim3(256), 0, st,
-                       (const T*)logits, a);
+      with_cut<false, kWhole>(
+          cut, 0, [&](auto nt, auto nv) { run(nt, nv, Int<0>{}); });
   });
   return (int)hipGetLastError();
 }
@@ -1135,7 +1228,7 @@ int dear_distill_fwd(hipStream_t st, int type, bool tail, const void* logits,
                          (RowStats*)stats, (Sums*)part};
   with_type(type, [&](auto zero) {
     using T = decltype(zero);
-    with_cut<false>(cut, 0, [&](auto nt, auto nv) {
+    with_cut<false, kSmallSlice>(cut, 0, [&](auto nt, auto nv) {
       constexpr int NT = decltype(nt)::value, NV = decltype(nv)::value;
       const dim3 grid(grid_for(rows * cut.slices)), block(NT);
       if (tail)
