@@ -500,11 +500,17 @@ __device__ __forceinline__ void leave_out(const LogprobArgs& a, int64_t row,
   }
 }
 
-// The numbers of a row from its sums, written by the `first` thread; log s to
-// all.
+// The token's logit; NaN of one outside of the vocabulary.
 template <typename T>
+__device__ __forceinline__ float logit_at(const LogprobArgs& a, int64_t token,
+                                          const T* z) {
+  return a.tokens && token >= 0 && token < a.V ? to_f(z[token]) : NAN;
+}
+
+// The numbers of a row from its sums and its token's logit, written by the
+// `first` thread; log s to all.
 __device__ __forceinline__ double finish_row(const LogprobArgs& a, int64_t row,
-                                             const T* z, const Sums& s,
+                                             float at, const Sums& s,
                                              bool first) {
   const float m = (float)s.m;
   const bool bad = no_distribution(m);
@@ -513,11 +519,7 @@ __device__ __forceinline__ double finish_row(const LogprobArgs& a, int64_t row,
   if (!first) return log_s;
   const double inv = 1.0 / (1.0 + others), h = log_s - kLn2 * s.e2 * inv;
   a.entropy[row] = (float)h;
-  if (a.tokens) {
-    const int64_t token = a.tokens[row];
-    const float at = token >= 0 && token < a.V ? to_f(z[token]) : NAN;
-    a.logprob[row] = (float)(((double)at - s.m) * a.inv_t - log_s);
-  }
+  if (a.tokens) a.logprob[row] = (float)(((double)at - s.m) * a.inv_t - log_s);
   if (a.stats)
     a.stats[row] = {m, bad ? NAN : (float)inv, (float)(h - log_s), 0.f};
   return log_s;
@@ -543,7 +545,8 @@ __global__ __launch_bounds__(NT, WHOLE ? 4 : 6) void logprobs_slice_kernel(
   for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
     const int64_t row = WHOLE || a.slices == 1 ? w : w / a.slices;
     const int base = (int)(w - row * a.slices) * a.per_slice;
-    if (a.tokens && a.tokens[row] == a.ignore) {
+    const int64_t token = a.tokens ? a.tokens[row] : 0;
+    if (a.tokens && token == a.ignore) {
       if constexpr (WHOLE) leave_out(a, row, threadIdx.x, NT);
       continue;
     }
@@ -551,6 +554,8 @@ __global__ __launch_bounds__(NT, WHOLE ? 4 : 6) void logprobs_slice_kernel(
     const int len = min(a.per_slice, a.V - base);
     Slice<T, NT, NV> s;
     s.load(z, len);
+    float at = NAN;
+    if constexpr (WHOLE) at = logit_at(a, token, z);
     const float mine = s.max();
     const float m = block_max<NT>(mine, wave_max);
     Sums r = {};
@@ -560,7 +565,7 @@ __global__ __launch_bounds__(NT, WHOLE ? 4 : 6) void logprobs_slice_kernel(
     if constexpr (!WHOLE) {
       if (threadIdx.x == 0) a.part[w] = r;
     } else if (threadIdx.x < 64) {       // while the others begin with the top
-      const double log_s = finish_row(a, row, z, r, threadIdx.x == 0);
+      const double log_s = finish_row(a, row, at, r, threadIdx.x == 0);
       if (threadIdx.x == 0) row_log_s = log_s;
     }
     if constexpr (TOP) {
@@ -586,18 +591,19 @@ __global__ __launch_bounds__(NT, WHOLE ? 4 : 6) void logprobs_slice_kernel(
 template <typename T>
 __global__ __launch_bounds__(256) void logprobs_finish_kernel(
     const T* __restrict__ logits, const LogprobArgs a) {
-  constexpr int kHeld = 1024;
+  constexpr int kHeld = 1024, kAhead = 8;
   __shared__ uint64_t held[4][kHeld];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < a.rows;
        row += (int64_t)gridDim.x * 4) {
-    if (a.tokens && a.tokens[row] == a.ignore) {
+    const int64_t token = a.tokens ? a.tokens[row] : 0;
+    if (a.tokens && token == a.ignore) {
       leave_out(a, row, lane, 64);
       continue;
     }
+    const float at = logit_at(a, token, logits + row * a.zs);
     const Sums s = join_sums(a.part + row * a.slices, a.slices, a.f);
-    const double log_s =
-        finish_row(a, row, logits + row * a.zs, s, lane == 0);
+    const double log_s = finish_row(a, row, at, s, lane == 0);
     if (a.k == 0) continue;              // there are no lists
     const uint64_t* lists = a.lists + row * a.slices * a.k;
     const int64_t entries = a.slices * a.k;
@@ -606,42 +612,46 @@ __global__ __launch_bounds__(256) void logprobs_finish_kernel(
     };
     if (a.slices == 1) {
       for (int i = lane; i < a.k; i += 64) put(i, lists[i]);
-    } else if (entries <= kHeld) {
-      // no better than the last of some list: not in the top. And k of them at
-      // least are as good as the worst of the lists' ceil(k / slices)-th. The
-      // others, little more than k, count how many are better than they
-      const int64_t deep = (a.k + a.slices - 1) / a.slices;
-      uint64_t last = 0, worst = ~0ull;
-      for (int64_t l = lane; l < a.slices; l += 64) {
-        last = max(last, lists[l * a.k + a.k - 1]);
-        worst = min(worst, lists[l * a.k + deep - 1]);
+      continue;
+    }
+    // No better than the last of some list: not in the top. And k of them at
+    // least are as good as the r-th best of the lists' d-th, r d >= k. The
+    // others, most often little more than k, count how many are better.
+    const int heads = (int)min(a.slices, (int64_t)64);
+    const int d = (a.k + heads - 1) / heads, r = (a.k + d - 1) / d;
+    uint64_t last = 0, head = 0;         // a lane's lists, the best of them
+    for (int64_t l = lane; l < a.slices; l += 64) {
+      last = max(last, lists[l * a.k + a.k - 1]);
+      head = max(head, lists[l * a.k + d - 1]);
+    }
+    int ahead = 0;
+    for (int j = 0; j < heads; ++j) ahead += __shfl(head, j) > head;
+    const uint64_t bar =
+        wave_reduce(max(last, ahead >= r - 1 ? head : 0), Larger{});
+    int64_t n = 0;
+    for (int64_t first = 0; first < entries; first += 64 * kAhead) {
+      uint64_t c[kAhead];                // loads that do not wait for another
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int64_t i = first + 64 * j + lane;
+        c[j] = i < entries ? lists[i] : 0;
       }
-      const uint64_t bar = max(wave_reduce(last, Larger{}),
-                               ~wave_reduce(~worst, Larger{}));
-      int n = 0;
-      for (int first = 0; first < entries; first += 64) {
-        const uint64_t c = first + lane < entries ? lists[first + lane] : 0;
-        const bool kept = c != 0 && c >= bar;
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const bool kept = c[j] != 0 && c[j] >= bar;
         const uint64_t all = __ballot(kept);
-        if (kept) held[wave][n + lanes_before(all)] = c;
+        const int64_t place = n + lanes_before(all);
+        if (kept && place < kHeld) held[wave][place] = c[j];
         n += __popcll(all);
       }
-      wave_fence();
+    }
+    wave_fence();
+    if (n <= kHeld) {
       for (int i = 0; i < n; i += 64) {
         const uint64_t mine = i + lane < n ? held[wave][i + lane] : 0;
         int rank = 0;
-        for (int first = 0; first < n; first += 64) {
-          // 64 of them in the lanes, one after the other to all
-          const uint64_t one = first + lane < n ? held[wave][first + lane] : 0;
-          const int many = min(64, n - first);
-          for (int j = 0; j < many; ++j) {
-            const uint64_t c =
-                (uint64_t)(uint32_t)__builtin_amdgcn_readlane(
-                    (int)(one >> 32), j) << 32 |
-                (uint32_t)__builtin_amdgcn_readlane((int)one, j);
-            rank += c > mine;
-          }
-        }
+#pragma unroll 4
+        for (int j = 0; j < (int)n; ++j) rank += held[wave][j] > mine;
         if (mine != 0 && rank < a.k) put(rank, mine);
       }
     } else {
@@ -1059,43 +1069,48 @@ Factor exp2_factor(double t) {
   return {(float)exact, exact, (exact / (double)(float)exact - 1.0) * kLn2};
 }
 
-// Slices of a row, of up to `most` 16-byte vectors; of up to 1024 where that
+// Slices of a row, of up to `most` 16-byte vectors; of up to `few` where that
 // would give fewer blocks than there are compute units. Smaller slices overlap
 // their phases better, larger ones leave fewer lists to make and join. Of 4096
 // and 2048 vectors, us: 614 of 4096 rows of 30528 fp32, no top, 28.8 and 25.0;
 // 4096 rows of 30528 bf16 with a top of 32 76.0 and 79.5, of 128 123 and 197;
 // distillation of the same with a tail 59.5 and 57.8, without 52.3 and 50.6.
-// One row of 30528 fp32 with a top of 8: 12.3 of 4096, 11.6 of 1024, 12.9 of
-// 512 vectors.
+// Few rows, of 4096 and 1024 vectors: 1 x 131072 bf16, top 8, 12.7 and 11.9,
+// top 64 16.5 and 31.4; 2 x 600011 fp32, top 16, 15.7 and 20.5, top 128 46 and
+// 130.
 struct Cut {
   int64_t each, slices;      // vectors of a slice, slices of a row
 };
-constexpr int kLargeSlice = 4096, kSmallSlice = 2048;
+constexpr int kLargeSlice = 4096, kSmallSlice = 2048, kFewRows = 1024;
 
-Cut cut_row(int64_t rows, int V, int per_vector, int64_t most) {
-  const int64_t vecs = (V + per_vector - 1) / per_vector;
-  if (rows * ((vecs + most - 1) / most) < 256) most = 1024;
-  const int64_t few = (vecs + most - 1) / most;
-  const int64_t each = (vecs + few - 1) / few;
+Cut cut_row(int64_t rows, int V, int per_vector, int64_t most, int64_t few) {
+  const int64_t vecs = ((int64_t)V + per_vector - 1) / per_vector;
+  if (rows * ((vecs + most - 1) / most) < 256) most = few;
+  const int64_t slices = (vecs + most - 1) / most;
+  const int64_t each = (vecs + slices - 1) / slices;
   return {each, (vecs + each - 1) / each};             // none of them empty
 }
 
 // Log probabilities of few rows: a block to each row if it can hold that, which
 // then needs no second kernel. A row of 30528 fp32 with a top of 8, us: 11.5 in
-// slices, 9.0 whole; 64 such rows 13.2 and 10.8.
+// slices, 8.5 whole; 64 such rows 13.2 and 10.1.
 constexpr int kWhole = 8192;
 Cut cut_logprobs(int type, int64_t rows, int V, int k) {
   const int E = type == kF32 ? 4 : 8;
   const int64_t vecs = ((int64_t)V + E - 1) / E;
   if (rows < 256 && vecs <= kWhole) return {vecs, 1};
-  return cut_row(rows, V, E, k ? kLargeSlice : kSmallSlice);
+  return k ? cut_row(rows, V, E, kLargeSlice, kLargeSlice)
+           : cut_row(rows, V, E, kSmallSlice, kFewRows);
+}
+Cut cut_distill(int type, int64_t rows, int V) {
+  return cut_row(rows, V, type == kF32 ? 4 : 8, kSmallSlice, kFewRows);
 }
 
 // Whether rows that are one slice are finished in their block: where all of
 // them run at once (4 waves on each SIMD) this saves a launch, and with more
 // the larger kernel's registers cost more than that. Us, apart and together:
-// 4096 x 1000 fp32, top 4, 14.7 and 10.7; 300 x 30528 bf16, top 32, 16.6 and
-// 15.1; 4096 x 30528 bf16, top 32, 76 and 90.
+// 4096 x 1000 fp32, top 4, 14.7 and 10.5; 300 x 30528 bf16, top 32, 16.6 and
+// 12.9; 4096 x 30528 bf16, top 32, 76 and 90.
 bool finish_there(const Cut& c, int64_t rows, int threads) {
   return c.slices == 1 && rows * threads <= 256 * 16 * 64;
 }
@@ -1115,13 +1130,15 @@ void with_cut(const Cut& c, int k, F f) {
       return;
     }
   }
+  if constexpr (MOST > kSmallSlice) {
+    if (c.each > kSmallSlice) {
+      f(Int<512>{}, Int<8>{});
+      return;
+    }
+  }
   if constexpr (TOP) {
     if (c.each <= 256) {
       f(Int<256>{}, Int<1>{});
-      return;
-    }
-    if (c.each > kSmallSlice) {
-      f(Int<512>{}, Int<8>{});
       return;
     }
   }
@@ -1145,7 +1162,7 @@ int64_t dear_logprobs_slices(int type, int64_t rows, int V, int k) {
   return cut_logprobs(type, rows, V, k).slices;
 }
 int64_t dear_distill_slices(int type, int64_t rows, int V) {
-  return cut_row(rows, V, per_vector(type), kSmallSlice).slices;
+  return cut_distill(type, rows, V).slices;
 }
 int64_t dear_slice_bytes() { return sizeof(Sums); }
 
@@ -1175,8 +1192,10 @@ int dear_logprobs_fwd(hipStream_t st, int type, const void* logits, int64_t zs,
         launch(nt, nv, top, Int<1>{});
         return;
       }
-      // rows that need a block of 1024 are always finished there
-      if constexpr (decltype(nt)::value < 1024) launch(nt, nv, top, Int<0>{});
+      // rows in longer slices are few, and were finished
+      if constexpr (decltype(nt)::value * decltype(nv)::value <=
+                    (decltype(top)::value ? kLargeSlice : kSmallSlice))
+        launch(nt, nv, top, Int<0>{});
       hipLaunchKernelGGL((logprobs_finish_kernel<T>),
                          dim3(grid_for((rows + 3) / 4)), dim3(256), 0, st,
                          (const T*)logits, a);
@@ -1221,7 +1240,7 @@ int dear_distill_fwd(hipStream_t st, int type, bool tail, const void* logits,
                      int64_t zs, const int64_t* ids, const float* teacher,
                      int64_t rows, int V, int k, double t, float* loss,
                      float* q, void* stats, void* part) {
-  const Cut cut = cut_row(rows, V, per_vector(type), kSmallSlice);
+  const Cut cut = cut_distill(type, rows, V);
   const DistillArgs a = {ids, teacher, zs, rows, V, k,
                          (int)(cut.each * per_vector(type)), cut.slices,
                          exp2_factor(t), t, 1.0 / t, loss, q,

@@ -532,6 +532,32 @@ def test_gpu_logprobs(R, V, top, T, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("R,V,top,T", [
+    # a block to each row, finished there and, of more rows, apart
+    (2, 30528, 0, 1.0), (255, 9001, 128, 1.0), (4200, 300, 5, 1.0),
+    (4200, 300, 0, 1.0), (1100, 1500, 40, 1.0), (1100, 5001, 0, 2.0),
+    (600, 16001, 20, 1.0),
+    # more slices than a wave has lanes
+    (1, 2200001, 128, 1.0), (1, 2200001, 7, 1.0), (1, 2200001, 0, 1.0)])
+def test_gpu_logprobs_blocks(R, V, top, T, dtype):
+    standard_logprobs(R, V, top, T, dtype, "cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [262144, 280001])
+def test_gpu_equal_lists(V):
+    """Slices that are alike but for one that is worse: next to nothing of
+    their lists can be left out."""
+    gen = torch.Generator().manual_seed(5)
+    one = torch.randn(2, 16384, generator=gen)
+    z = one.repeat(1, 18)[:, :V].contiguous()
+    z[:, 16384:32768] -= 30.0
+    tokens = torch.tensor([7, V - 1]).cuda()
+    compare_logprobs(z.cuda(), tokens, make_ups(2, 128, gen, "cuda"), 128, 1.0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("R,V,K,T", [
