@@ -140,6 +140,13 @@ __device__ __forceinline__ void load_columns(float (&v)[NV * E], const void* p,
   }
 }
 
+// Bound by memory: 16384 x 1024, a bf16 branch on an fp32 residual, takes 23 us
+// (7.3 TB/s, part of it from the last-level cache; 34 us where nothing of it is
+// there), 4096 x 768 fp32 5.9 us. One row takes 2.5 us, a launch's own time.
+// 256 threads hold one to sixteen rows: a wave to a row of up to 1024 elements
+// needs no barrier, and the lanes' sums go through DPP, not LDS. Against one
+// block to a row with elements loaded one by one: 254 us for this pass and the
+// backward's, 83 now.
 template <typename TX, typename TR, typename TY, bool RES, int G, int NV>
 __global__ __launch_bounds__(G > 256 ? G : 256, 4) void ln_fwd_kernel(
     const TX* __restrict__ x, int64_t xs, const TR* __restrict__ r, int64_t rs,
@@ -198,6 +205,12 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 4) void ln_fwd_kernel(
   }
 }
 
+// Bound by memory as well: the same case takes 46 us (5.9 TB/s; 56 us where
+// nothing is cached), 4096 x 768 fp32 14 us. Few blocks, each of many rows, as
+// many as leave 256 records: a record per row would be as many bytes again as
+// the gradient. Gradients that are stored past the caches are written no
+// faster here (93 us for a pass instead of 83): what reads them next then has
+// to fetch them.
 template <typename TX, typename TR, typename TY, bool RES, int G, int NV>
 __global__ __launch_bounds__(G > 512 ? G : G > 64 ? 256 : 512,
                              G > 512 ? 4 : 2)
@@ -304,6 +317,8 @@ void ln_bwd_kernel(
 }
 
 // Adds up the records: 64 columns to a block of 1024, 16 threads to a column.
+// No atomics, so that the result does not depend on the order of the blocks.
+// Bound by latency: 256 records of 2 x 1024 columns, 2 MB, take 4 us.
 __global__ __launch_bounds__(1024) void ln_records_kernel(
     const float* __restrict__ records, int n, int H, void* __restrict__ dw,
     void* __restrict__ db, int wtype) {
