@@ -257,28 +257,32 @@ __device__ __forceinline__ float wave_sort(float v) {
   return exchange<64, 32>(v);
 }
 
+// A wave's ceil(k / waves)-th best of its threads' maxima, written before the
+// waves meet for the row's maximum.
+template <int NT>
+__device__ __forceinline__ void put_floor(float mine, int k,
+                                          float* wave_floor) {
+  const int each = (k + NT / 64 - 1) / (NT / 64);
+  const float bar = each == 1 ? wave_reduce(mine, Max{})
+                              : __shfl(wave_sort(mine), each - 1);
+  if ((threadIdx.x & 63) == 0) wave_floor[threadIdx.x >> 6] = bar;
+}
+
 // The k best of a slice into found[0..n), in no order; every thread gets n.
 // k is at most NT. Each of the NT / 64 waves has ceil(k / waves) elements that
-// reach the smallest of the waves' such maxima of threads: k elements at least
-// reach it, and about twice k do if the row is in no order. Two steps collect
-// them: the 16-byte pieces that have one, known by their maxima, and then a
-// thread for each element of those, from memory again.
+// reach the smallest of the waves' floors: k elements at least reach it, and
+// about twice k do if the row is in no order. Two steps collect them: the
+// 16-byte pieces that have one, known by their maxima, and then a thread for
+// each element of those, from memory again. count[0] and [1] are zero.
 template <typename T, int NT, int NV>
 __device__ int slice_top(const Slice<T, NT, NV>& s, const T* z, int len,
-                         int base, int k, float mine, bool has_nan,
-                         uint64_t* found, int* count, float* wave_floor,
-                         int* scratch) {
+                         int base, int k, bool has_nan, uint64_t* found,
+                         int* count, const float* wave_floor, int* scratch) {
   constexpr int W = NT / 64, E = kVec<T>;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
   uint16_t* pieces = reinterpret_cast<uint16_t*>(found + kCandidates);
   float bar = NAN;
   if (!has_nan) {
-    const int each = (k + W - 1) / W;
-    bar = each == 1 ? wave_reduce(mine, Max{})
-                    : __shfl(wave_sort(mine), each - 1);
-    if (lane == 0) wave_floor[wave] = bar;
-    if (threadIdx.x < 2) count[threadIdx.x] = 0;
-    __syncthreads();
     bar = wave_floor[0];
 #pragma unroll
     for (int i = 1; i < W; ++i) bar = fminf(bar, wave_floor[i]);
@@ -336,9 +340,13 @@ __device__ __forceinline__ void ranked(const uint64_t* found, int n, int k,
   for (int first = 0; first < n; first += NT >> share) {
     const int i = first + ((int)threadIdx.x >> share);
     const uint64_t mine = i < n ? found[i] : 0;
-    float better = 0.f;
-    for (int j = sub; j < n; j += 1 << share)
-      better += found[j] > mine ? 1.f : 0.f;
+    int count = 0, j = sub;
+    for (; j + (3 << share) < n; j += 4 << share) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) count += found[j + (u << share)] > mine;
+    }
+    for (; j < n; j += 1 << share) count += found[j] > mine;
+    float better = (float)count;
     if (share > 0) better = sum_of(lanes<1>(better));
     if (share > 1) better = sum_of(lanes<2>(better));
     if (share > 2) better = sum_of(lanes<4>(better));
@@ -543,8 +551,9 @@ __device__ __forceinline__ void put_top(const LogprobArgs& a, int64_t place,
 // vector unit alike, which is busy for three quarters of that: a conversion,
 // a subtraction, a product, exp2, two sums and the maximum for each element.
 // 68 us with a top of 32, where the phases of a block wait for each other, and
-// 115 with one of 128. The row is never read again from memory but for some
-// hundred pieces that may hold one of the top.
+// 107 with one of 128, 30 of it the ranking's reads of LDS. The row is never
+// read again from memory but for some hundred pieces that may hold one of the
+// top.
 template <typename T, int NT, int NV, bool TOP, bool WHOLE>
 __global__ __launch_bounds__(NT, WHOLE ? 4 : 6) void logprobs_slice_kernel(
     const T* __restrict__ logits, const LogprobArgs a) {
@@ -570,6 +579,10 @@ __global__ __launch_bounds__(NT, WHOLE ? 4 : 6) void logprobs_slice_kernel(
     float at = NAN;
     if constexpr (WHOLE) at = logit_at(a, token, z);
     const float mine = s.max();
+    if constexpr (TOP) {
+      put_floor<NT>(mine, min(a.k, len), wave_floor);
+      if (threadIdx.x < 2) count[threadIdx.x] = 0;
+    }
     const float m = block_max<NT>(mine, wave_max);
     Sums r = {};
     if (!no_distribution(m))
@@ -583,7 +596,7 @@ __global__ __launch_bounds__(NT, WHOLE ? 4 : 6) void logprobs_slice_kernel(
     }
     if constexpr (TOP) {
       const int k = min(a.k, len);
-      const int n = slice_top(s, z, len, base, k, mine, m != m, found, count,
+      const int n = slice_top(s, z, len, base, k, m != m, found, count,
                               wave_floor, scratch);
       if constexpr (WHOLE) {             // k is a.k
         const double log_s = row_log_s;
@@ -1156,7 +1169,7 @@ Cut cut_row(int64_t rows, int V, int per_vector, int64_t most, int64_t few) {
 
 // Log probabilities of few rows: a block to each row if it can hold that, which
 // then needs no second kernel. A row of 30528 fp32 with a top of 8, us: 11.5 in
-// slices, 8.5 whole; 64 such rows 13.2 and 10.1.
+// slices, 8.3 whole; 64 such rows 13.2 and 9.7.
 constexpr int kWhole = 8192;
 Cut cut_logprobs(int type, int64_t rows, int V, int k) {
   const int E = type == kF32 ? 4 : 8;
