@@ -3,9 +3,11 @@
 // token or a small batch the host's work, not the kernel, is the cost.
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 
 int64_t dear_ln_blocks(int, int64_t, int);
 int dear_ln_fwd(hipStream_t, int, int, int, const void*, int64_t, const void*,
@@ -88,6 +90,30 @@ variable_list once(variable_list grads, const char* name) {
   return (*node)(std::move(grads));
 }
 
+// Whether a leaf's gradient is accumulated on another stream than the current
+// one, as it is while a graph that was made there lives.
+bool accumulates_elsewhere(const Tensor& leaf) {
+  if (!leaf.defined() || !leaf.requires_grad() || !leaf.is_leaf()) return false;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
+  const auto stream = node ? node->stream() : std::nullopt;
+  const c10::impl::VirtualGuardImpl guard(leaf.device().type());
+  return stream && *stream != guard.getStream(leaf.device());
+}
+
+// A captured backward pass cannot hand a gradient to a stream outside of the
+// capture; the process would end where it tries to.
+void check_capture(std::initializer_list<Tensor> leaves, hipStream_t stream,
+                   const char* name) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  check_launch((int)hipStreamIsCapturing(stream, &status));
+  if (status == hipStreamCaptureStatusNone) return;
+  for (const auto& t : leaves)
+    TORCH_CHECK(!accumulates_elsewhere(t), name, ": a backward pass is being "
+                "captured while a graph of the same leaf that was made on "
+                "another stream is alive; free that one first, or make it on "
+                "the stream of the capture");
+}
+
 bool wants_grad(std::initializer_list<Tensor> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const auto& t : ts)
@@ -147,6 +173,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
                  &stats = saved[3];
     const Tensor& affine = w.defined() ? w : saved[4];
     const c10::DeviceGuard guard(x.device());
+    check_capture({x, affine, res}, stream_of(x), "layer_norm");
     const auto [rows, width] = ln_shape(x);
     // the node has an edge for each tensor that was given
     const bool has_b = ctx->saved_data["bias"].toBool();
@@ -320,6 +347,7 @@ struct LogprobsFn : torch::autograd::Function<LogprobsFn> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &tokens = saved[1];
     const c10::DeviceGuard guard(logits.device());
+    check_capture({logits}, stream_of(logits), "token_logprobs");
     const int64_t top = ctx->saved_data["top"].toInt();
     const size_t at0 = tokens.defined() ? 1 : 0;
     const Tensor dlp = tokens.defined() ? up_of(up, 0) : Tensor();
@@ -408,6 +436,7 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &ids = saved[1];
     const c10::DeviceGuard guard(logits.device());
+    check_capture({logits}, stream_of(logits), "topk_distill_loss");
     const auto z = logit_rows(logits);
     Tensor dz = at::empty(logits.sizes(), logits.options());
     if (z.rows) {

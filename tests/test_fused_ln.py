@@ -367,6 +367,27 @@ def test_gpu_streams_and_graph():
 
 
 @pytest.mark.gpu
+def test_gpu_capture_beside_a_live_eager_graph_is_refused():
+    x, w, b, _, dy = make(8, 64, F32, F32, F32, "cuda")
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    alive = layer_norm(*leaves)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = layer_norm(*leaves)
+        with pytest.raises(RuntimeError, match="alive"):
+            torch.autograd.grad(y, leaves, dy)
+    want = torch.autograd.grad(alive, leaves, dy)
+    del alive, y
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(layer_norm(*leaves), leaves, dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, v) for g, v in zip(got, want))
+
+
+@pytest.mark.gpu
 def test_gpu_second_derivative_is_refused():
     x, w, b, _, _ = make(4, 16, F32, None, F32, "cuda")
     x.requires_grad_(True)

@@ -743,6 +743,30 @@ def test_gpu_streams_and_graph():
 
 
 @pytest.mark.gpu
+def test_gpu_capture_beside_a_live_eager_graph_is_refused():
+    z, gen = make_logits(5, 300, F32, "cuda")
+    z.requires_grad_(True)
+    ids, lp = make_teacher(z.detach(), 4, 1.0, gen)
+    for loss in (lambda: token_logprobs(z, ids[:, 0].contiguous()).logprob,
+                 lambda: topk_distill_loss(z, ids, lp)):
+        alive, up = loss(), torch.ones(5, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = loss()
+            with pytest.raises(RuntimeError, match="alive"):
+                torch.autograd.grad(y, z, up)
+        want, = torch.autograd.grad(alive, z, up)
+        del alive, y
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(loss(), z, up)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
 def test_gpu_second_derivative_is_refused():
     z = torch.randn(3, 9, device="cuda", requires_grad=True)
     tokens = torch.zeros(3, dtype=torch.long, device="cuda")
