@@ -17,12 +17,11 @@ int dear_ln_bwd(hipStream_t, int, int, int, const void*, int64_t, const void*,
                 int64_t, const void*, int64_t, const void*, const float*,
                 const float*, void*, void*, void*, void*, float*, int, int64_t,
                 int);
-int64_t dear_logprobs_slices(int, int64_t, int, int);
-int64_t dear_distill_slices(int, int64_t, int);
-int64_t dear_slice_bytes();
+int64_t dear_logprobs_work(int, int64_t, int, int);
+int64_t dear_distill_work(int, int64_t, int);
 int dear_logprobs_fwd(hipStream_t, int, const void*, int64_t, const int64_t*,
                       int64_t, int64_t, int, int, double, float*, float*,
-                      float*, int64_t*, void*, void*, void*);
+                      float*, int64_t*, void*, void*);
 int dear_logprobs_bwd(hipStream_t, int, const void*, int64_t, const int64_t*,
                       const int64_t*, const void*, const float*, const float*,
                       const float*, void*, int64_t, int, int, double);
@@ -274,10 +273,8 @@ void check_logits(const Tensor& t, const char* name) {
                     "tokens");
 }
 
-// What the slices of rows leave for the kernel that joins them
-Tensor slice_records(const Tensor& logits, int64_t rows, int64_t slices) {
-  return at::empty({rows * slices, dear_slice_bytes()},
-                   logits.options().dtype(at::kByte));
+Tensor workspace(const Tensor& like, int64_t bytes) {
+  return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 
 // logprob (where there are tokens), entropy, and with top > 0 the top's log
@@ -301,17 +298,13 @@ variable_list logprobs_forward(const Tensor& logits, const Tensor& tokens,
   if (z.rows) {
     const Tensor tok = tokens.defined() ? tokens.contiguous() : Tensor();
     const int type = type_code(logits, "logits");
-    const Tensor part = slice_records(
-        logits, z.rows,
-        dear_logprobs_slices(type, z.rows, z.width, (int)top));
-    Tensor lists;
-    if (top)
-      lists = at::empty({part.size(0), top}, logits.options().dtype(at::kLong));
+    const Tensor work = workspace(
+        logits, dear_logprobs_work(type, z.rows, z.width, (int)top));
     check_launch(dear_logprobs_fwd(
         stream_of(logits), type, data(z.t),
         z.t.dim() == 2 ? z.t.stride(0) : 0, idata(tok), ignore, z.rows,
         z.width, (int)top, t, fdata(lp), fdata(h), fdata(tlp), idata(tid),
-        stats ? data(*stats) : nullptr, data(part), data(lists)));
+        stats ? data(*stats) : nullptr, data(work)));
   }
   variable_list out;
   if (tokens.defined()) out.push_back(lp);
@@ -394,29 +387,29 @@ variable_list token_logprobs(const Tensor& logits,
 }
 
 // ------------------------------------------------------------ distillation
+// `kept`: for the backward pass, four numbers a row, and behind them the
+// teacher's shares
 Tensor distill_forward(const Tensor& logits, const Tensor& ids,
-                       const Tensor& teacher, double t, bool tail, Tensor* q,
-                       Tensor* stats) {
+                       const Tensor& teacher, double t, bool tail,
+                       Tensor* kept) {
   const c10::DeviceGuard guard(logits.device());
   const auto z = logit_rows(logits);
   const auto fopt = logits.options().dtype(at::kFloat);
   const int64_t k = ids.size(-1);
   Tensor loss = at::empty(logits.sizes().slice(0, logits.dim() - 1), fopt);
-  if (stats) {
-    *q = at::empty({z.rows, k}, fopt);
-    *stats = at::empty({z.rows, 4}, fopt);
-  }
+  if (kept) *kept = at::empty({z.rows * (4 + k)}, fopt);
   if (z.rows) {
     const Tensor idc = ids.contiguous();
     const Tensor tc = teacher.to(at::kFloat).contiguous();
     const int type = type_code(logits, "logits");
-    const Tensor part = slice_records(
-        logits, z.rows, dear_distill_slices(type, z.rows, z.width));
+    const Tensor work = workspace(
+        logits, dear_distill_work(type, z.rows, z.width));
+    float* stats = kept ? fdata(*kept) : nullptr;
     check_launch(dear_distill_fwd(
         stream_of(logits), type, tail, data(z.t),
         z.t.dim() == 2 ? z.t.stride(0) : 0, idata(idc), fdata(tc), z.rows,
-        z.width, (int)k, t, fdata(loss), q ? fdata(*q) : nullptr,
-        stats ? data(*stats) : nullptr, data(part)));
+        z.width, (int)k, t, fdata(loss),
+        stats ? stats + z.rows * 4 : nullptr, stats, data(work)));
   }
   return loss;
 }
@@ -425,9 +418,9 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& logits,
                         const Tensor& ids, const Tensor& teacher, double t,
                         bool tail) {
-    Tensor q, stats;
-    Tensor loss = distill_forward(logits, ids, teacher, t, tail, &q, &stats);
-    ctx->save_for_backward({logits, ids, q, stats});
+    Tensor kept;
+    Tensor loss = distill_forward(logits, ids, teacher, t, tail, &kept);
+    ctx->save_for_backward({logits, ids, kept});
     ctx->saved_data["t"] = t;
     return loss;
   }
@@ -443,8 +436,9 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
       const Tensor idc = ids.contiguous(), g = up[0].contiguous();
       check_launch(dear_distill_bwd(
           stream_of(logits), type_code(logits, "logits"), data(z.t),
-          z.t.dim() == 2 ? z.t.stride(0) : 0, idata(idc), fdata(saved[2]),
-          data(saved[3]), fdata(g), data(dz), z.rows, z.width,
+          z.t.dim() == 2 ? z.t.stride(0) : 0, idata(idc),
+          fdata(saved[2]) + z.rows * 4, data(saved[2]), fdata(g), data(dz),
+          z.rows, z.width,
           (int)ids.size(-1), ctx->saved_data["t"].toDouble()));
     }
     return once({dz, Tensor(), Tensor(), Tensor(), Tensor()},
@@ -469,7 +463,7 @@ Tensor topk_distill_loss(const Tensor& logits, const Tensor& ids,
   TORCH_CHECK_VALUE(logits.is_cuda(),
                     "topk_distill_loss: logits are not on a GPU");
   if (!wants_grad({logits}))
-    return distill_forward(logits, ids, teacher, t, tail, nullptr, nullptr);
+    return distill_forward(logits, ids, teacher, t, tail, nullptr);
   return DistillFn::apply(logits, ids, teacher, t, tail);
 }
 

@@ -1233,26 +1233,36 @@ int per_vector(int type) { return type == kF32 ? 4 : 8; }
 
 }  // namespace
 
-// Slices of a row, and bytes of the record that each leaves.
-int64_t dear_logprobs_slices(int type, int64_t rows, int V, int k) {
-  return cut_logprobs(type, rows, V, k).slices;
+// Bytes that a forward pass leaves for the kernel that joins the slices; 0
+// where there is none.
+int64_t dear_logprobs_work(int type, int64_t rows, int V, int k) {
+  const Cut cut = cut_logprobs(type, rows, V, k);
+  bool whole = false;
+  auto ask = [&](auto nt, auto) {
+    whole = finish_there(cut, rows, decltype(nt)::value);
+  };
+  if (k) with_cut<true, kWhole>(cut, k, ask);
+  else with_cut<false, kWhole>(cut, 0, ask);
+  return whole ? 0
+               : rows * cut.slices *
+                     (int64_t)(sizeof(Sums) + k * sizeof(uint64_t));
 }
-int64_t dear_distill_slices(int type, int64_t rows, int V) {
-  return cut_distill(type, rows, V).slices;
+int64_t dear_distill_work(int type, int64_t rows, int V) {
+  return rows * cut_distill(type, rows, V).slices * (int64_t)sizeof(Sums);
 }
-int64_t dear_slice_bytes() { return sizeof(Sums); }
 
 int dear_logprobs_fwd(hipStream_t st, int type, const void* logits, int64_t zs,
                       const int64_t* tokens, int64_t ignore, int64_t rows,
                       int V, int k, double t, float* logprob, float* entropy,
-                      float* top_lp, int64_t* top_ids, void* stats, void* part,
-                      void* lists) {
+                      float* top_lp, int64_t* top_ids, void* stats,
+                      void* work) {
   const Cut cut = cut_logprobs(type, rows, V, k);
+  Sums* part = (Sums*)work;              // and behind the records the lists
   const LogprobArgs a = {tokens, zs, ignore, rows, V, k,
                          (int)(cut.each * per_vector(type)), cut.slices,
                          exp2_factor(t), 1.0 / t, logprob, entropy,
-                         top_lp, top_ids, (RowStats*)stats, (Sums*)part,
-                         (uint64_t*)lists};
+                         top_lp, top_ids, (RowStats*)stats, part,
+                         (uint64_t*)(part + rows * cut.slices)};
   with_type(type, [&](auto zero) {
     using T = decltype(zero);
     auto launch = [&](auto nt, auto nv, auto top, auto whole) {
@@ -1315,12 +1325,12 @@ int dear_logprobs_bwd(hipStream_t st, int type, const void* logits, int64_t zs,
 int dear_distill_fwd(hipStream_t st, int type, bool tail, const void* logits,
                      int64_t zs, const int64_t* ids, const float* teacher,
                      int64_t rows, int V, int k, double t, float* loss,
-                     float* q, void* stats, void* part) {
+                     float* q, void* stats, void* work) {
   const Cut cut = cut_distill(type, rows, V);
   const DistillArgs a = {ids, teacher, zs, rows, V, k,
                          (int)(cut.each * per_vector(type)), cut.slices,
                          exp2_factor(t), t, 1.0 / t, loss, q,
-                         (RowStats*)stats, (Sums*)part};
+                         (RowStats*)stats, (Sums*)work};
   with_type(type, [&](auto zero) {
     using T = decltype(zero);
     with_cut<false, kSmallSlice>(cut, 0, [&](auto nt, auto nv) {
