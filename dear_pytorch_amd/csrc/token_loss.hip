@@ -973,7 +973,10 @@ __global__ __launch_bounds__(256) void distill_finish_kernel(
 }
 
 // ----------------------------------------------------------------- backward
-// A block of 256 takes 512 vectors of one row.
+// A block of 256 takes 512 vectors of one row. The last row comes first: what
+// the forward pass has read last is still in the last-level cache (4096 x 30528
+// bf16, 250 MB, in a pass of forward and backward: 88 us in the rows' order, 81
+// in this one).
 constexpr int kBwdThreads = 256;
 constexpr int kBwdVectors = 2;
 template <typename T>
@@ -1039,8 +1042,8 @@ __global__ __launch_bounds__(kBwdThreads) void logprobs_bwd_kernel(
     float inv_t) {
   __shared__ int token_in_top;
   const int tid = threadIdx.x;
-  for (int64_t w = blockIdx.x; w < rows * pieces; w += gridDim.x) {
-    const int64_t row = w / pieces;
+  for (int64_t i = blockIdx.x; i < rows * pieces; i += gridDim.x) {
+    const int64_t w = rows * pieces - 1 - i, row = w / pieces;
     const int base = (int)(w - row * pieces) * kBwdTokens<T>;
     const int len = min(kBwdTokens<T>, V - base);
     const T* z = logits + row * zs + base;
@@ -1096,7 +1099,7 @@ __global__ __launch_bounds__(kBwdThreads) void logprobs_bwd_kernel(
   }
 }
 
-// Bound by memory: 4096 x 30528 bf16, 86 us (5.8 TB/s); 614 rows of fp32,
+// Bound by memory: 4096 x 30528 bf16, 81 us (6.2 TB/s); 614 rows of fp32,
 // 150 MB in all, 23.5 us (6.4 TB/s).
 template <typename T, bool STREAM>
 __global__ __launch_bounds__(kBwdThreads) void distill_bwd_kernel(
@@ -1106,8 +1109,8 @@ __global__ __launch_bounds__(kBwdThreads) void distill_bwd_kernel(
     T* __restrict__ dz, int64_t rows, int V, int64_t pieces, int k, float c,
     float t) {
   const int tid = threadIdx.x;
-  for (int64_t w = blockIdx.x; w < rows * pieces; w += gridDim.x) {
-    const int64_t row = w / pieces;
+  for (int64_t i = blockIdx.x; i < rows * pieces; i += gridDim.x) {
+    const int64_t w = rows * pieces - 1 - i, row = w / pieces;
     const int base = (int)(w - row * pieces) * kBwdTokens<T>;
     const int len = min(kBwdTokens<T>, V - base);
     const T* z = logits + row * zs + base;
