@@ -419,6 +419,26 @@ def test_cpu_odd_teachers():
     odd_teachers("cpu")
 
 
+def long_lists_with_repeats(dev):
+    """Up to 128 entries, some of them one token's: side by side, 64 apart,
+    three times, and all of them."""
+    z, gen = make_logits(6, 5000, F32, dev, seed=3)
+    up = torch.rand(6, generator=gen).to(dev)
+    for K in (60, 100, 128):
+        ids, lp = make_teacher(z, K, 1.0, gen)
+        ids[0, 1] = ids[0, 0]
+        ids[1, K - 1] = ids[1, K - 65 if K > 64 else 0]
+        ids[2, 7] = ids[2, K // 2] = ids[2, K - 2]
+        ids[3, :] = ids[3, :1]
+        ids[4, K // 2:] = ids[4, :K - K // 2].flip(0)
+        for tail in (False, True):
+            compare_distill(z, ids, lp - 1.0, up, 1.0, tail)
+
+
+def test_cpu_long_lists_with_repeats():
+    long_lists_with_repeats("cpu")
+
+
 def test_gradients_against_differences():
     gen = torch.Generator().manual_seed(3)
     z = torch.randn(4, 9, generator=gen, dtype=torch.double) \
@@ -587,6 +607,11 @@ def test_gpu_unknown_tokens():
 @pytest.mark.gpu
 def test_gpu_odd_teachers():
     odd_teachers("cuda")
+
+
+@pytest.mark.gpu
+def test_gpu_long_lists_with_repeats():
+    long_lists_with_repeats("cuda")
 
 
 @pytest.mark.gpu
