@@ -23,12 +23,12 @@
 // Precision: exp(t) is exp2((z - m) c) with c = log2(e) / T: the difference is
 // taken first, so that it is 0 for the largest element and errors stay small
 // whatever the size of m. (One fma of z c - m c instead was no faster: 53.7 us
-// for 52.8 at 4096 x 30528 bf16.) What c loses in fp32, at most 2^-25 of t, is
+// for 52.8 at 4096 x 30528 bf16.) What c loses in fp32, at most 2^-24 of t, is
 // the same for all elements; where the entropy's sum is at hand it is taken out
 // of s in fp64. (Distillation has no such sum, and would take 67 us for 55 with
-// one.) Sums of a wave are fp32, those over waves fp64. The elements equal to m are counted apart: s = 1 + r for a
-// row that is sure of its token, and log1p(r) keeps the digits of a
-// probability near one.
+// one.) Sums of a wave are fp32, those over waves fp64. The elements equal to m
+// are counted apart: s = 1 + r for a row that is sure of its token, and
+// log(1 + r) keeps the digits of a probability near one.
 #include <hip/hip_runtime.h>
 
 #include "lm_common.h"
@@ -431,7 +431,7 @@ __device__ __forceinline__ Sums slice_sums(Slice<T, NT, NV>& s, float m,
         r.n_in += p[4];
       }
     }
-    // exp2(y c_exact / c) of every element, to first order (2^-25 squared)
+    // exp2(y c_exact / c) of every element, to first order (2^-24 squared)
     if constexpr (ENT) r.rest += f.lost * r.e2;
   }
   r.m = m;
