@@ -195,9 +195,18 @@ def _distill_torch(logits, ids, teacher, temperature, tail):
     if tail:
         named = torch.zeros(lp.shape, dtype=torch.int32, device=lp.device)
         named = named.scatter_add_(-1, at, present.int()) > 0
-        left = lp.masked_fill(named, -math.inf)
-        some = (left.detach() > -math.inf).any(-1)
-        out = torch.where(some[..., None], left, 0.0).logsumexp(-1)
+        # log p_t from the distances to the outside's own largest logit: next
+        # to that of a far mask, the sum's logarithm would have no digits
+        with torch.no_grad():
+            far = x.masked_fill(named, -math.inf).amax(-1, keepdim=True)
+            some = far[..., 0] != -math.inf
+        left = torch.where(some[..., None], x - far, 0.0) / temperature
+        out = left.masked_fill(named & some[..., None], -math.inf) \
+            .logsumexp(-1)
+        best = x.argmax(-1, keepdim=True)
+        out = out + ((far - x.gather(-1, best)) / temperature
+                     + lp.gather(-1, best))[..., 0]
+        out = torch.where(some, out, 0.0)
         loss = loss + torch.where(some & (rest != 0.0), rest * (
             rest.masked_fill(rest == 0.0, 1.0).log() - out), 0.0)
     # a student's row that is no distribution: NaN, whatever the teacher says
