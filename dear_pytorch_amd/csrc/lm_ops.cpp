@@ -387,8 +387,8 @@ variable_list token_logprobs(const Tensor& logits,
 }
 
 // ------------------------------------------------------------ distillation
-// `kept`: for the backward pass, four numbers a row, and behind them the
-// teacher's shares
+// `kept`: for the backward pass, four numbers a row, and behind them the named
+// tokens' gradients
 Tensor distill_forward(const Tensor& logits, const Tensor& ids,
                        const Tensor& teacher, double t, bool tail,
                        Tensor* kept) {

@@ -11,7 +11,11 @@
 //   dz_j = 1/T (sum_i c_i (1[id_i = j] - p_j) - dH p_j (l_j + H))
 //   dz_j = T dloss (W p_j - sum_{id_k = j} q_k - [j not named] p_j q_t / p_t),
 //   W = sum q_k + q_t. Where the student gives nothing to the tokens outside
-//   (p_t = 0) the term of q_t is left out of loss and W.
+//   (all of their logits are -inf) the term of q_t is left out of loss and W.
+// With a tail the outside has a largest logit m_o of its own, and its sum
+// s_o = sum exp((z_j - m_o) / T) is relative to that: however far below m it
+// lies, log p_t = (m_o - m) / T + log s_o - log s, and p_j q_t / p_t is
+// exp((z_j - m_o) / T) q_t / s_o.
 //
 // Forward: a block takes a slice of one row into registers, 16 bytes a load,
 // passes over it there (the maximum, then the sums, then the top) and leaves a
@@ -65,7 +69,15 @@ __device__ __forceinline__ float logit_of(uint64_t c) {
 // What a row leaves for its backward pass: p_j = exp2((z_j - m) c) inv_s.
 // inv_s == 0: the row was not looked at, its gradient is zero.
 struct RowStats {
-  float m, inv_s, a, b;
+  float m, inv_s, a, unused;
+};
+
+// The same of a distillation's row. With m the largest logit of the tokens
+// outside (without a tail: of all) the gradient is exp2((z_j - m) c) outside,
+// in units of T dloss; the named tokens have theirs from the forward pass.
+// live == 0: the row was not looked at.
+struct DistillRow {
+  float m, outside, live, unused;
 };
 
 // log2(e) / T, what fp32 leaves of it, and ln 2 times what that loses.
@@ -75,10 +87,10 @@ struct Factor {
 };
 
 // The sums of a slice or of a row, relative to its maximum m: n elements are
-// equal to m, `rest` and e2 (of e log2 e) are over the others. With a tail
-// these are the elements outside, and n_in and in are over the named ones.
+// equal to m, `rest` and e2 (of e log2 e) are over the others. With a tail all
+// of this is over the elements outside.
 struct Sums {
-  double m, n, rest, e2, n_in, in;
+  double m, n, rest, e2;
 };
 
 __device__ __forceinline__ bool no_distribution(float m) {
@@ -357,13 +369,10 @@ __device__ __forceinline__ void ranked(const uint64_t* found, int n, int k,
 
 // ------------------------------------------------------ sums of one slice
 // Adds up one slice against the maximum m (not NaN, finite). ENT: e2 too.
-// TAIL: without the elements of `named`, a bit for each of the thread; `in` and
-// `n_in` are the thread's share of these. Results in every thread of the first
-// wave.
-template <typename T, int NT, int NV, bool ENT, bool TAIL>
+// Results in every thread of the first wave.
+template <typename T, int NT, int NV, bool ENT>
 __device__ __forceinline__ Sums slice_sums(Slice<T, NT, NV>& s, float m,
-                                           Factor f, uint64_t named, float in,
-                                           float n_in, float (*scratch)[6]) {
+                                           Factor f, float (*scratch)[3]) {
   constexpr int W = NT / 64, E = kVec<T>;
   float rest = 0.f, e2 = 0.f, n = 0.f;
   auto add = [&](int v) {
@@ -378,20 +387,7 @@ __device__ __forceinline__ Sums slice_sums(Slice<T, NT, NV>& s, float m,
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     s.fresh(v);
-    if constexpr (TAIL) {
-      // some pieces of most waves have a named element: these, and the ones
-      // equal to m, become -inf, which adds nothing
-      uint32_t mask = (uint32_t)(named >> v * E) & ((1u << E) - 1u);
-      if (s.vmax[v] == m) {
-        uint32_t largest = 0;
-#pragma unroll
-        for (int j = 0; j < E; ++j) largest |= s.at(v, j) == m ? 1u << j : 0u;
-        n += (float)__popc(largest & ~mask);
-        mask |= largest;
-      }
-      if (mask) s.drop(v, mask);
-      add(v);
-    } else if (s.vmax[v] != m) {
+    if (s.vmax[v] != m) {
       add(v);
     } else {
 #pragma unroll
@@ -410,13 +406,9 @@ __device__ __forceinline__ Sums slice_sums(Slice<T, NT, NV>& s, float m,
   rest = wave_reduce(rest, Add{});
   n = wave_reduce(n, Add{});
   if constexpr (ENT) e2 = wave_reduce(e2, Add{});
-  if constexpr (TAIL) {
-    in = wave_reduce(in, Add{});
-    n_in = wave_reduce(n_in, Add{});
-  }
   if ((threadIdx.x & 63) == 0) {
     float* p = scratch[threadIdx.x >> 6];
-    p[0] = rest; p[1] = n; p[2] = e2; p[3] = in; p[4] = n_in;
+    p[0] = rest; p[1] = n; p[2] = e2;
   }
   __syncthreads();
   Sums r = {};
@@ -426,10 +418,6 @@ __device__ __forceinline__ Sums slice_sums(Slice<T, NT, NV>& s, float m,
       r.rest += p[0];
       r.n += p[1];
       if constexpr (ENT) r.e2 += p[2];
-      if constexpr (TAIL) {
-        r.in += p[3];
-        r.n_in += p[4];
-      }
     }
     // exp2(y c_exact / c) of every element, to first order (2^-24 squared)
     if constexpr (ENT) r.rest += f.lost * r.e2;
@@ -460,14 +448,11 @@ __device__ __forceinline__ Sums join_sums(const Sums& mine, const Sums* part,
       r.n += p.n;
       r.rest += p.rest;
       r.e2 += p.e2;
-      r.n_in += p.n_in;
-      r.in += p.in;
     } else if (p.m > -INFINITY) {
       const double y = (p.m - (double)m) * f.exact, g = exp2(y);
       const double all = p.n + p.rest;
       r.rest += g * all;
       r.e2 += g == 0.0 ? 0.0 : g * (p.e2 + y * all);
-      r.in += g * (p.n_in + p.in);
     }
   };
   if (lane < ns) add(mine);
@@ -476,14 +461,10 @@ __device__ __forceinline__ Sums join_sums(const Sums& mine, const Sums* part,
     r.n += __shfl_xor(r.n, o);
     r.rest += __shfl_xor(r.rest, o);
     r.e2 += __shfl_xor(r.e2, o);
-    r.n_in += __shfl_xor(r.n_in, o);
-    r.in += __shfl_xor(r.in, o);
   }
   r.n = __shfl(r.n, 0);
   r.rest = __shfl(r.rest, 0);
   r.e2 = __shfl(r.e2, 0);
-  r.n_in = __shfl(r.n_in, 0);
-  r.in = __shfl(r.in, 0);
   return r;
 }
 
@@ -559,7 +540,7 @@ template <typename T, int NT, int NV, bool TOP, bool WHOLE>
 __global__ __launch_bounds__(NT, WHOLE ? 4 : 6) void logprobs_slice_kernel(
     const T* __restrict__ logits, const LogprobArgs a) {
   __shared__ float wave_max[NT / 64], wave_floor[NT / 64];
-  __shared__ float sums[NT / 64][6];
+  __shared__ float sums[NT / 64][3];
   __shared__ int scratch[NT / 64];
   __shared__ uint64_t found[TOP ? kCandidates + kPieces / 4 : 1];
   __shared__ int count[2];
@@ -587,7 +568,7 @@ __global__ __launch_bounds__(NT, WHOLE ? 4 : 6) void logprobs_slice_kernel(
     const float m = block_max<NT>(mine, wave_max);
     Sums r = {};
     if (!no_distribution(m))
-      r = slice_sums<T, NT, NV, true, false>(s, m, a.f, 0, 0.f, 0.f, sums);
+      r = slice_sums<T, NT, NV, true>(s, m, a.f, sums);
     r.m = m;
     if constexpr (!WHOLE) {
       if (threadIdx.x == 0) a.part[w] = r;
@@ -720,8 +701,8 @@ struct DistillArgs {
   int64_t slices;
   Factor f;
   double t, inv_t;
-  float *loss, *q_out;
-  RowStats* stats;
+  float *loss, *named_out;   // and the named tokens' gradients, a.k a row
+  DistillRow* stats;
   Sums* part;
 };
 
@@ -744,13 +725,14 @@ struct Entries {
   }
 };
 
-// Whether a lane's id is another entry's as well. All write their number into
-// the slot of their id; whose number is read there is done, and so are the
-// entries with the same id. The others, of another id in the same slot, go on.
+// Whether a lane's id is another entry's as well, and which of the entries of
+// one id stands for it. All write their number into the slot of their id; whose
+// number is read there is done, and so are the entries with the same id. The
+// others, of another id in the same slot, go on.
 // 614 rows of 64 entries: 2.5 us less than comparing each id with all others.
 constexpr int kSlots = 2048;
 template <int N>
-__device__ __forceinline__ bool named_twice(const int (&id)[N],
+__device__ __forceinline__ bool named_twice(const int (&id)[N], bool (&one)[N],
                                             uint8_t* slots) {
   const int lane = threadIdx.x & 63;
   bool twice = false, open[N];
@@ -759,6 +741,7 @@ __device__ __forceinline__ bool named_twice(const int (&id)[N],
   for (int e = 0; e < N; ++e) {
     slot[e] = ((uint32_t)id[e] * 0x9e3779b1u) >> 21;     // under kSlots
     open[e] = true;
+    one[e] = false;
   }
   bool go_on = true;
   while (__any(go_on)) {
@@ -776,7 +759,8 @@ __device__ __forceinline__ bool named_twice(const int (&id)[N],
         if (owner >= 64) theirs = other;
       }
       if (open[e] && theirs == id[e]) {
-        twice |= owner != lane + 64 * e;
+        one[e] = owner == lane + 64 * e;
+        twice |= !one[e];
         open[e] = false;
       }
       go_on |= open[e];
@@ -802,9 +786,47 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a,
     if constexpr (N > 1) top = MaxNan{}(top, t.lp[1]);
     top = wave_reduce(top, MaxNan{});
   }
-  const float m = (float)s.m;
+  // The absent entries are no id's; of ids past 32 bits the loss is NaN anyway.
+  int id[N];
+  bool one[N], twice = false;
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    id[e] = t.id[e] < 0 ? -1 - lane - 64 * e : (int)t.id[e];
+  if (TAIL || a.stats) twice = __any(named_twice<N>(id, one, slots));
+  // the largest logit of the tokens outside, and of the row
+  const float m_out = (float)s.m;
+  float m = m_out;
+  if constexpr (TAIL) {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      m = MaxNan{}(m, t.id[e] < 0 ? -INFINITY : t.z[e]);
+    m = wave_reduce(m, MaxNan{});
+  }
+  const bool bad = no_distribution(m);
+  double x[N] = {}, in = 0.0, n_in = 0.0;    // exp of the entries, each id once
+  if (!bad && (TAIL || a.stats)) {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (t.id[e] >= 0) x[e] = exp(((double)t.z[e] - (double)m) * a.inv_t);
+  }
+  double n = s.n, less = s.rest, gap = 0.0, shrink = 1.0;
   const double outside = s.n + s.rest;
-  const double others = (s.rest + s.in) + ((s.n + s.n_in) - 1.0);
+  if constexpr (TAIL) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      if (t.id[e] < 0 || !one[e]) continue;
+      if (t.z[e] == m) n_in += 1.0;
+      else in += x[e];
+    }
+    wave_sum(in, n_in);
+    if (m_out < m) {
+      gap = ((double)m_out - (double)m) * a.inv_t;
+      shrink = exp(gap);
+      n = 0.0;
+      less = shrink * outside;
+    }
+  }
+  const double others = (less + in) + ((n + n_in) - 1.0);
   const double sum = 1.0 + others, log_s = log_1p(others);
   double q[N], all_q = 0.0, total = 0.0, rest = 0.0;
 #pragma unroll
@@ -815,7 +837,7 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a,
     if (t.z[e] != t.z[e])                    // no such token, or a NaN
       total = NAN;
     else if (q[e] != 0.0)
-      total += q[e] * (lq - (((double)t.z[e] - s.m) * a.inv_t - log_s));
+      total += q[e] * (lq - (((double)t.z[e] - (double)m) * a.inv_t - log_s));
   }
   wave_sum(all_q, total);
   if constexpr (TAIL) {
@@ -827,57 +849,55 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a,
     for (int e = 0; e < N; ++e) q[e] *= by;
     all_q = 1.0;
   }
-  double share = all_q, shift = 0.0;
-  if (TAIL && rest != 0.0 && outside > 0.0) {
+  double share = all_q, tail = 0.0;
+  if (TAIL && rest != 0.0 && m_out != -INFINITY) {
     share += rest;
-    shift = rest * sum / outside;        // q_t / p_t
-    total += rest * log(shift);
+    tail = rest / outside;               // q_t / s_o
+    total += rest * (log(tail * sum) - gap);
   }
-  if (no_distribution(m)) total = NAN;
+  if (bad) total = NAN;
   if (lane == 0) a.loss[row] = (float)(total * a.t * a.t);
   if (!a.stats) return;
+  const double inv = total != total ? NAN : 1.0 / sum;
   if (lane == 0)
-    a.stats[row] = {m, total != total ? NAN : (float)(1.0 / sum),
-                    (float)share, (float)(share - shift)};
-  // An id that is named more than once: each of its entries gets the sum. The
-  // absent ones are no id's; of ids past 32 bits the loss is NaN anyway.
-  int id[N];
-#pragma unroll
-  for (int e = 0; e < N; ++e)
-    id[e] = t.id[e] < 0 ? -1 - lane - 64 * e : (int)t.id[e];
-  if (__any(named_twice<N>(id, slots))) {
+    a.stats[row] = {m_out == -INFINITY ? 0.f : m_out,
+                    (float)(share * (shrink * inv) - tail), 1.f, 0.f};
+  // an id that is named more than once: each of its entries gets the sum
+  if (twice) {
     double sum_q[N] = {};
     for (int i = 0; i < 64; ++i)
 #pragma unroll
       for (int e = 0; e < N; ++e) {
-        const int one = __shfl(id[e], i);
+        const int theirs = __shfl(id[e], i);
         const double share_of_one = __shfl(q[e], i);
 #pragma unroll
         for (int d = 0; d < N; ++d)
-          if (one == id[d]) sum_q[d] += share_of_one;
+          if (theirs == id[d]) sum_q[d] += share_of_one;
       }
 #pragma unroll
     for (int e = 0; e < N; ++e) q[e] = sum_q[e];
   }
 #pragma unroll
   for (int e = 0; e < N; ++e)
-    if (lane + 64 * e < a.k) a.q_out[row * a.k + lane + 64 * e] = (float)q[e];
+    if (lane + 64 * e < a.k)
+      a.named_out[row * a.k + lane + 64 * e] =
+          (float)(share * (x[e] * inv) - q[e]);
 }
 
 // 4096 x 30528 bf16, 32 entries, with the kernel that joins the slices: 48 us
-// without a tail, 55 with one (4.5 TB/s). With a tail the elements that are
-// named have to be left out of the sum exactly; taking them from the sum
-// afterwards would leave nothing of a small tail. They are known by a bit for
-// each element of a thread, which cost less than comparing the ids (67 us).
+// without a tail; with one, where nothing is cached, 61 (4.1 TB/s). With a tail
+// the elements that are named have to be left out of maximum and sum exactly:
+// taking them from the sum afterwards, or summing the others relative to them,
+// would leave nothing of a small tail. They are known by a bit for each element
+// of a thread, which cost less than comparing the ids (67 us).
 template <typename T, int NT, int NV, bool TAIL>
 __global__ __launch_bounds__(NT, 6) void distill_slice_kernel(
     const T* __restrict__ logits, const DistillArgs a) {
   constexpr int E = kVec<T>;
   constexpr int kOwn = (kMaxTop + NT - 1) / NT;     // entries of a thread
   __shared__ float wave_max[NT / 64];
-  __shared__ float sums[NT / 64][6];
+  __shared__ float sums[NT / 64][3];
   __shared__ uint64_t masks[TAIL ? NT : 1];         // a bit for each element
-  __shared__ int twice;
   const int64_t work = a.rows * a.slices;
   const int tid = threadIdx.x;
   for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
@@ -892,52 +912,33 @@ __global__ __launch_bounds__(NT, 6) void distill_slice_kernel(
       id[e] = i < a.k ? ids[i] : -1;
       live |= id[e] >= 0;
     }
-    if constexpr (TAIL) {
-      masks[tid] = 0;
-      if (tid == 0) twice = 0;
-    }
+    if constexpr (TAIL) masks[tid] = 0;
     if (!__syncthreads_or(live)) continue;
     const T* z = logits + row * a.zs + base;
     const int len = min(a.per_slice, a.V - base);
     Slice<T, NT, NV> s;
     s.load(z, len);
-    float own[kOwn];
-    bool mine_named[kOwn];
     if constexpr (TAIL) {
+      // the named ones become -inf, which adds nothing
 #pragma unroll
       for (int e = 0; e < kOwn; ++e) {
         const int64_t at = id[e] - base;
-        mine_named[e] = at >= 0 && at < len;
-        own[e] = 0.f;
-        if (!mine_named[e]) continue;
-        own[e] = to_f(z[at]);
+        if (at < 0 || at >= len) continue;
         const int piece = (int)at / E, bit = piece / NT * E + (int)at % E;
-        const uint64_t one = 1ull << bit;
-        if (atomicOr((unsigned long long*)&masks[piece % NT], one) & one)
-          twice = 1;
+        atomicOr((unsigned long long*)&masks[piece % NT], 1ull << bit);
       }
-    }
-    const float mine = s.max();
-    const float m = block_max<NT>(mine, wave_max);   // synchronises
-    Sums r = {};
-    if (!no_distribution(m)) {
-      float in = 0.f, n_in = 0.f;
-      uint64_t named = 0;
-      if constexpr (TAIL) {
-        named = masks[tid];
+      __syncthreads();
+      const uint64_t named = masks[tid];
 #pragma unroll
-        for (int e = 0; e < kOwn; ++e) {
-          // of an id that is named twice the first entry counts
-          if (twice && mine_named[e])
-            for (int i = 0; i < tid + e * NT; ++i)
-              if (ids[i] == id[e]) mine_named[e] = false;
-          if (!mine_named[e]) continue;
-          if (own[e] == m) n_in += 1.f;
-          else in += __builtin_amdgcn_exp2f((own[e] - m) * a.f.c);
-        }
+      for (int v = 0; v < NV; ++v) {
+        const uint32_t mask = (uint32_t)(named >> v * E) & ((1u << E) - 1u);
+        if (mask) s.drop(v, mask);
       }
-      r = slice_sums<T, NT, NV, false, TAIL>(s, m, a.f, named, in, n_in, sums);
     }
+    const float m = block_max<NT>(s.max(), wave_max);     // synchronises
+    Sums r = {};
+    if (!no_distribution(m))
+      r = slice_sums<T, NT, NV, false>(s, m, a.f, sums);
     r.m = m;
     if (tid == 0) a.part[w] = r;
     __syncthreads();
@@ -964,7 +965,7 @@ __global__ __launch_bounds__(256) void distill_finish_kernel(
       if (lane == 0) a.loss[row] = 0.f;
       if (a.stats) {
         if (lane == 0) a.stats[row] = {0.f, 0.f, 0.f, 0.f};
-        for (int i = lane; i < a.k; i += 64) a.q_out[row * a.k + i] = 0.f;
+        for (int i = lane; i < a.k; i += 64) a.named_out[row * a.k + i] = 0.f;
       }
       continue;
     }
@@ -1105,8 +1106,8 @@ __global__ __launch_bounds__(kBwdThreads) void logprobs_bwd_kernel(
 template <typename T, bool STREAM>
 __global__ __launch_bounds__(kBwdThreads) void distill_bwd_kernel(
     const T* __restrict__ logits, int64_t zs,
-    const int64_t* __restrict__ ids, const float* __restrict__ q,
-    const RowStats* __restrict__ stats, const float* __restrict__ d_loss,
+    const int64_t* __restrict__ ids, const float* __restrict__ named,
+    const DistillRow* __restrict__ stats, const float* __restrict__ d_loss,
     T* __restrict__ dz, int64_t rows, int V, int64_t pieces, int k, float c,
     float t) {
   const int tid = threadIdx.x;
@@ -1116,24 +1117,21 @@ __global__ __launch_bounds__(kBwdThreads) void distill_bwd_kernel(
     const int len = min(kBwdTokens<T>, V - base);
     const T* z = logits + row * zs + base;
     T* out = dz + row * V + base;
-    const RowStats s = stats[row];
-    if (s.inv_s == 0.f) {
+    const DistillRow s = stats[row];
+    if (s.live == 0.f) {
       zero_piece<STREAM>(out, len);
       continue;
     }
-    const float g = d_loss[row] * t, outside = s.inv_s * s.b * g;
+    const float g = d_loss[row] * t, outside = s.outside * g;
+    // with a tail what this gives the named tokens may be anything
     map_piece<STREAM>(z, out, len, [&](float v) {
       return __builtin_amdgcn_exp2f((v - s.m) * c) * outside;
     });
     __syncthreads();
     if (tid < k) {
       const int64_t id = ids[row * k + tid];
-      if (id >= base && id - base < len) {
-        const int i = (int)(id - base);
-        const float p =
-            __builtin_amdgcn_exp2f((to_f(z[i]) - s.m) * c) * s.inv_s;
-        out[i] = static_cast<T>((p * s.a - q[row * k + tid]) * g);
-      }
+      if (id >= base && id - base < len)
+        out[(int)(id - base)] = static_cast<T>(named[row * k + tid] * g);
     }
   }
 }
@@ -1329,12 +1327,12 @@ int dear_logprobs_bwd(hipStream_t st, int type, const void* logits, int64_t zs,
 int dear_distill_fwd(hipStream_t st, int type, bool tail, const void* logits,
                      int64_t zs, const int64_t* ids, const float* teacher,
                      int64_t rows, int V, int k, double t, float* loss,
-                     float* q, void* stats, void* work) {
+                     float* named, void* stats, void* work) {
   const Cut cut = cut_distill(type, rows, V);
   const DistillArgs a = {ids, teacher, zs, rows, V, k,
                          (int)(cut.each * per_vector(type)), cut.slices,
-                         exp2_factor(t), t, 1.0 / t, loss, q,
-                         (RowStats*)stats, (Sums*)work};
+                         exp2_factor(t), t, 1.0 / t, loss, named,
+                         (DistillRow*)stats, (Sums*)work};
   with_type(type, [&](auto zero) {
     using T = decltype(zero);
     with_cut<false, kSmallSlice>(cut, 0, [&](auto nt, auto nv) {
@@ -1360,7 +1358,7 @@ int dear_distill_fwd(hipStream_t st, int type, bool tail, const void* logits,
 }
 
 int dear_distill_bwd(hipStream_t st, int type, const void* logits, int64_t zs,
-                     const int64_t* ids, const float* q, const void* stats,
+                     const int64_t* ids, const float* named, const void* stats,
                      const float* d_loss, void* dz, int64_t rows, int V, int k,
                      double t) {
   with_type(type, [&](auto zero) {
@@ -1369,8 +1367,8 @@ int dear_distill_bwd(hipStream_t st, int type, const void* logits, int64_t zs,
     auto launch = [&](auto stream) {
       hipLaunchKernelGGL((distill_bwd_kernel<T, decltype(stream)::value>),
                          dim3(grid_for(rows * pieces)), dim3(kBwdThreads), 0,
-                         st, (const T*)logits, zs, ids, q,
-                         (const RowStats*)stats, d_loss, (T*)dz, rows, V,
+                         st, (const T*)logits, zs, ids, named,
+                         (const DistillRow*)stats, d_loss, (T*)dz, rows, V,
                          pieces, k, exp2_factor(t).c, (float)t);
     };
     rows * V * (int64_t)sizeof(T) > kStreamBytes ? launch(Int<1>{})

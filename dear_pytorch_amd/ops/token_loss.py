@@ -143,8 +143,9 @@ def topk_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor,
     tail=False: the teacher is their softmax over the named tokens, so that
     its logits divided by the temperature do as well. tail=True: what their
     exponentials leave up to one is the share of all other tokens together,
-    and is compared with what the student gives to these together; where the
-    student gives them nothing at all that term is left out.
+    and is compared with what the student gives to these together, however
+    little that is; where it gives them nothing at all (all of their logits are
+    -inf) that term is left out.
 
     The teacher is constant: its tensors must not ask for a gradient.
     """

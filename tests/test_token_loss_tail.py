@@ -197,3 +197,42 @@ def test_cpu_a_tail_in_its_numbers():
     # 1/2 log 1/2 + 1/2 (log 1/2 - (log 3 - 100))
     assert abs(loss[0].item() - (math.log(0.5) + 50 - 0.5 * math.log(3))) < 1e-5
     assert (g[0] - torch.tensor([0.5] + [-1 / 6] * 3)).abs().max() < 1e-6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("where", ["all", "first", "last"])
+@pytest.mark.parametrize("V,K,T", [
+    (4, 1, 1.0), (40, 5, 0.1), (300, 17, 2.0), (5000, 128, 0.05),
+    (30528, 32, 1.0), (30528, 100, 0.1), (70001, 9, 1.0), (131075, 1, 0.5)])
+def test_gpu_far(V, K, T, where, dtype):
+    far(V, K, T, dtype, "cuda", where)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [2, 40, 9000, 30528, 70001])
+def test_gpu_lowest(V, dtype):
+    lowest(V, dtype, "cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [300, 30528])
+def test_gpu_one_of_many(V, dtype):
+    one_and_many(V, dtype, "cuda")
+
+
+@pytest.mark.gpu
+def test_gpu_a_tail_is_the_cpu_paths():
+    z, ids, lp = far_rows(30528, 12, 1.0, F32, "cpu")
+    ids[3, 4:] = ids[3, :1]                     # named more than once
+    ids[6, 6:] = -1
+    up = ups(len(GAPS), "cpu")
+    loss, g = run_distill(z, ids, lp, up, tail=True)
+    got, dz = run_distill(z.cuda(), ids.cuda(), lp.cuda(), up.cuda(),
+                          tail=True)
+    want = exact(z, ids, lp, 1.0, True, up)
+    for a, b, key in ((got, loss, "loss"), (dz, g, "dlogits")):
+        check(a.cpu(), *want[key], what=key)
+        check(b, *want[key], what=key)
