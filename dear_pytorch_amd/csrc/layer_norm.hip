@@ -12,6 +12,13 @@
 // bytes as a stored z would cost, and no rounding of z in between. Sums and
 // statistics are fp32; results are rounded once, to their own type.
 //
+// A mean in fp32 is off by some 2^-22 of itself, which may be more than the
+// row's whole spread. What it is off by is the mean of the distances to it: that
+// is summed with their squares, and kept as a second number. Where it is more
+// than an eighth of the spread, the sum of squares says too little, and another
+// round is taken from the mean that both numbers give; the distances to that are
+// exact, and those of equal elements are 0.
+//
 // A row lies in the registers of a group of 16, 32, 64, 256 or 1024 threads,
 // up to 16 elements of each, so that it is read once. Groups go round the rows
 // with their columns' weights, and in the backward their columns' sums of
@@ -107,6 +114,26 @@ struct GroupSum {
   }
 };
 
+// What a row leaves for its backward pass: its mean is the sum of two numbers.
+// [3][rows]
+struct RowNorm {
+  float mean, off, rstd;
+};
+__device__ __forceinline__ void put_stats(float* stats, int64_t rows,
+                                          int64_t row, float mean, float off,
+                                          float rstd) {
+  stats[row] = mean;
+  stats[rows + row] = off;
+  stats[2 * rows + row] = rstd;
+}
+__device__ __forceinline__ RowNorm get_stats(const float* stats, int64_t rows,
+                                             int64_t row) {
+  return {stats[row], stats[rows + row], stats[2 * rows + row]};
+}
+__device__ __forceinline__ float norm_of(float z, const RowNorm& s) {
+  return ((z - s.mean) - s.off) * s.rstd;
+}
+
 // E elements a chunk: 16 bytes of the narrowest type.
 template <typename TX>
 constexpr int kChunk = kVec<TX>;
@@ -151,8 +178,8 @@ template <typename TX, typename TR, typename TY, bool RES, int G, int NV>
 __global__ __launch_bounds__(G > 256 ? G : 256, 4) void ln_fwd_kernel(
     const TX* __restrict__ x, int64_t xs, const TR* __restrict__ r, int64_t rs,
     const void* __restrict__ w, const void* __restrict__ b, int wtype,
-    TY* __restrict__ y, float* __restrict__ mean_out,
-    float* __restrict__ rstd_out, int64_t rows, int H, float eps) {
+    TY* __restrict__ y, float* __restrict__ stats, int64_t rows, int H,
+    float eps) {
   constexpr int E = kChunk<TX>, NT = G > 256 ? G : 256, N = NV * E;
   __shared__ float scratch[2][G > 64 ? G / 64 : 1][2];
   GroupSum<G> group_sum{scratch};
@@ -179,29 +206,54 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 4) void ln_fwd_kernel(
         z[c * E + j] = v;
         s += v;
       }
-    // divided, so that the mean of equal elements is the element
-    const float mean = group_sum(s) / (float)H;
-    float q = 0.f;
+    float mean = group_sum(s) / (float)H, off = 0.f, q = 0.f;
+    auto inside = [&](int c, int j) { return first + c * G * E + j < H; };
 #pragma unroll
     for (int c = 0; c < NV; ++c)
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const float d = z[c * E + j] - mean;
-        q += first + c * G * E + j < H ? d * d : 0.f;
+        const float d = inside(c, j) ? z[c * E + j] - mean : 0.f;
+        z[c * E + j] = d;
+        off += d;
+        q = fmaf(d, d, q);
       }
-    const float rstd = 1.0f / sqrtf(group_sum(q) / (float)H + eps);
+    group_sum(off, q);
+    // the same in all threads of the group, which meet again in the sums
+    const bool again = 64.f * off * (off / (float)H) > q;
+    off /= (float)H;
+    float var = q / (float)H - off * off;
+    if (again) {
+      const float better = mean + off, step = better - mean;
+      mean = better;
+      off = q = 0.f;
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          if (inside(c, j)) z[c * E + j] -= step;
+          off += z[c * E + j];
+        }
+      off = group_sum(off) / (float)H;
+#pragma unroll
+      for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const float d = inside(c, j) ? z[c * E + j] - off : 0.f;
+          q = fmaf(d, d, q);
+        }
+      var = group_sum(q) / (float)H;
+    }
+    const float rstd = 1.0f / sqrtf(var + eps);
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
 #pragma unroll
       for (int j = 0; j < E; ++j)
-        z[c * E + j] = fmaf((z[c * E + j] - mean) * rstd, wv[c * E + j],
+        z[c * E + j] = fmaf((z[c * E + j] - off) * rstd, wv[c * E + j],
                             bv[c * E + j]);
       store_chunk<TY, E>(y + row * H, first + c * G * E, H, z + c * E);
     }
-    if (mean_out && threadIdx.x % G == 0) {
-      mean_out[row] = mean;
-      rstd_out[row] = rstd;
-    }
+    if (stats && threadIdx.x % G == 0)
+      put_stats(stats, rows, row, mean, off, rstd);
   }
 }
 
@@ -217,8 +269,7 @@ __global__ __launch_bounds__(G > 512 ? G : G > 64 ? 256 : 512,
 void ln_bwd_kernel(
     const TX* __restrict__ x, int64_t xs, const TR* __restrict__ r, int64_t rs,
     const TY* __restrict__ dy, int64_t dys, const void* __restrict__ w,
-    int wtype, const float* __restrict__ mean_in,
-    const float* __restrict__ rstd_in, TX* __restrict__ dx,
+    int wtype, const float* __restrict__ stats, TX* __restrict__ dx,
     TR* __restrict__ dr, float* __restrict__ records, int64_t rows, int H) {
   constexpr int E = kChunk<TX>, N = NV * E;
   constexpr int NT = G > 512 ? G : G > 64 ? 256 : 512;
@@ -239,7 +290,7 @@ void ln_bwd_kernel(
       if constexpr (RES) cr[c].load(r + row * rs, first + c * G * E, H);
       cg[c].load(dy + row * dys, first + c * G * E, H);
     }
-    const float mean = mean_in[row], rstd = rstd_in[row];
+    const RowNorm stat = get_stats(stats, rows, row);
     float n[N], g[N], sg = 0.f, sgn = 0.f;
 #pragma unroll
     for (int c = 0; c < NV; ++c)
@@ -248,7 +299,7 @@ void ln_bwd_kernel(
         const int i = c * E + j;
         float z = cx[c].at(j);
         if constexpr (RES) z += cr[c].at(j);
-        n[i] = (z - mean) * rstd;
+        n[i] = norm_of(z, stat);
         const float up = cg[c].at(j);
         aw[i] = fmaf(up, n[i], aw[i]);
         ab[i] += up;
@@ -264,7 +315,7 @@ void ln_bwd_kernel(
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const int i = c * E + j;
-        g[i] = rstd * (g[i] - sg - n[i] * sgn);
+        g[i] = stat.rstd * (g[i] - sg - n[i] * sgn);
       }
       if (dx) store_chunk<TX, E>(dx + row * H, first + c * G * E, H, g + c * E);
       if constexpr (RES)
@@ -352,33 +403,33 @@ template <typename TX, typename TR, typename TY, bool RES>
 __global__ __launch_bounds__(kLongThreads) void ln_fwd_long_kernel(
     const TX* __restrict__ x, int64_t xs, const TR* __restrict__ r, int64_t rs,
     const void* __restrict__ w, const void* __restrict__ b, int wtype,
-    TY* __restrict__ y, float* __restrict__ mean_out,
-    float* __restrict__ rstd_out, int64_t rows, int H, float eps) {
-  __shared__ float scratch[kLongThreads / 64];
+    TY* __restrict__ y, float* __restrict__ stats, int64_t rows, int H,
+    float eps) {
+  __shared__ double scratch[kLongThreads / 64];
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const TX* xr = x + row * xs;
     const TR* rr = RES ? r + row * rs : nullptr;
-    float s = 0.f;
+    double s = 0.0, v = 0.0;
     for (int i = threadIdx.x; i < H; i += kLongThreads)
       s += load_z<TX, TR, RES>(xr, rr, i);
-    const float mean = block_reduce(s, Add{}, scratch) / (float)H;
-    float v = 0.f;
+    const double mean = block_reduce(s, Add{}, scratch) / H;
     for (int i = threadIdx.x; i < H; i += kLongThreads) {
-      const float d = load_z<TX, TR, RES>(xr, rr, i) - mean;
+      const double d = load_z<TX, TR, RES>(xr, rr, i) - mean;
       v += d * d;
     }
-    const float var = block_reduce(v, Add{}, scratch) / (float)H;
-    const float rstd = 1.0f / sqrtf(var + eps);
+    v = block_reduce(v, Add{}, scratch) / H;
+    RowNorm stat;
+    stat.mean = (float)mean;
+    stat.off = (float)(mean - (double)stat.mean);
+    stat.rstd = 1.0f / sqrtf((float)v + eps);
     for (int i = threadIdx.x; i < H; i += kLongThreads) {
-      float n = (load_z<TX, TR, RES>(xr, rr, i) - mean) * rstd;
+      float n = norm_of(load_z<TX, TR, RES>(xr, rr, i), stat);
       if (w) n *= load_as_float(w, wtype, i);
       if (b) n += load_as_float(b, wtype, i);
       y[row * H + i] = static_cast<TY>(n);
     }
-    if (mean_out && threadIdx.x == 0) {
-      mean_out[row] = mean;
-      rstd_out[row] = rstd;
-    }
+    if (stats && threadIdx.x == 0)
+      put_stats(stats, rows, row, stat.mean, stat.off, stat.rstd);
   }
 }
 
@@ -386,29 +437,28 @@ template <typename TX, typename TR, typename TY, bool RES>
 __global__ __launch_bounds__(kLongThreads) void ln_bwd_long_kernel(
     const TX* __restrict__ x, int64_t xs, const TR* __restrict__ r, int64_t rs,
     const TY* __restrict__ dy, int64_t dys, const void* __restrict__ w,
-    int wtype, const float* __restrict__ mean_in,
-    const float* __restrict__ rstd_in, TX* __restrict__ dx,
+    int wtype, const float* __restrict__ stats, TX* __restrict__ dx,
     TR* __restrict__ dr, int64_t rows, int H) {
   __shared__ float scratch[kLongThreads / 64];
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const TX* xr = x + row * xs;
     const TR* rr = RES ? r + row * rs : nullptr;
     const TY* gr = dy + row * dys;
-    const float mean = mean_in[row], rstd = rstd_in[row];
+    const RowNorm stat = get_stats(stats, rows, row);
     float sg = 0.f, sgn = 0.f;
     for (int i = threadIdx.x; i < H; i += kLongThreads) {
       float g = to_f(gr[i]);
       if (w) g *= load_as_float(w, wtype, i);
       sg += g;
-      sgn += g * ((load_z<TX, TR, RES>(xr, rr, i) - mean) * rstd);
+      sgn += g * norm_of(load_z<TX, TR, RES>(xr, rr, i), stat);
     }
     sg = block_reduce(sg, Add{}, scratch) / (float)H;
     sgn = block_reduce(sgn, Add{}, scratch) / (float)H;
     for (int i = threadIdx.x; i < H; i += kLongThreads) {
       float g = to_f(gr[i]);
       if (w) g *= load_as_float(w, wtype, i);
-      const float n = (load_z<TX, TR, RES>(xr, rr, i) - mean) * rstd;
-      const float dz = rstd * (g - sg - n * sgn);
+      const float n = norm_of(load_z<TX, TR, RES>(xr, rr, i), stat);
+      const float dz = stat.rstd * (g - sg - n * sgn);
       if (dx) dx[row * H + i] = static_cast<TX>(dz);
       if (RES && dr) dr[row * H + i] = static_cast<TR>(dz);
     }
@@ -419,9 +469,8 @@ __global__ __launch_bounds__(kLongThreads) void ln_bwd_long_kernel(
 template <typename TX, typename TR, typename TY, bool RES>
 __global__ __launch_bounds__(256) void ln_dw_long_kernel(
     const TX* __restrict__ x, int64_t xs, const TR* __restrict__ r, int64_t rs,
-    const TY* __restrict__ dy, int64_t dys, const float* __restrict__ mean_in,
-    const float* __restrict__ rstd_in, float* __restrict__ records,
-    int64_t rows, int H) {
+    const TY* __restrict__ dy, int64_t dys, const float* __restrict__ stats,
+    float* __restrict__ records, int64_t rows, int H) {
   __shared__ float sw[4][64], sb[4][64];
   const int lane = threadIdx.x & 63, sub = threadIdx.x >> 6;
   for (int64_t at = (int64_t)blockIdx.y * 64; at < H;
@@ -434,7 +483,7 @@ __global__ __launch_bounds__(256) void ln_dw_long_kernel(
         const float g = to_f(dy[row * dys + col]);
         const float z = load_z<TX, TR, RES>(x + row * xs,
                                             RES ? r + row * rs : nullptr, col);
-        aw += g * ((z - mean_in[row]) * rstd_in[row]);
+        aw += g * norm_of(z, get_stats(stats, rows, row));
         ab += g;
       }
     sw[sub][lane] = aw;
@@ -492,13 +541,13 @@ int64_t bwd_blocks(int64_t rows, int H, int chunk) {
 
 template <typename TX, typename TR, typename TY, bool RES>
 void fwd(hipStream_t st, const void* x, int64_t xs, const void* r, int64_t rs,
-         const void* w, const void* b, int wtype, void* y, float* mean,
-         float* rstd, int64_t rows, int H, float eps) {
+         const void* w, const void* b, int wtype, void* y, float* stats,
+         int64_t rows, int H, float eps) {
   if (group_of(H, kChunk<TX>) == 0) {
     hipLaunchKernelGGL((ln_fwd_long_kernel<TX, TR, TY, RES>),
                        dim3(at_most(rows, kMaxBlocks)), dim3(kLongThreads), 0,
                        st, (const TX*)x, xs, (const TR*)r, rs, w, b, wtype,
-                       (TY*)y, mean, rstd, rows, H, eps);
+                       (TY*)y, stats, rows, H, eps);
     return;
   }
   with_group<kChunk<TX>>(H, [&](auto g, auto nv) {
@@ -508,34 +557,34 @@ void fwd(hipStream_t st, const void* x, int64_t xs, const void* r, int64_t rs,
     hipLaunchKernelGGL((ln_fwd_kernel<TX, TR, TY, RES, G, NV>),
                        dim3(at_most(blocks, 2048)), dim3(NT), 0, st,
                        (const TX*)x, xs, (const TR*)r, rs, w, b, wtype, (TY*)y,
-                       mean, rstd, rows, H, eps);
+                       stats, rows, H, eps);
   });
 }
 
 template <typename TX, typename TR, typename TY, bool RES>
 void bwd(hipStream_t st, const void* x, int64_t xs, const void* r, int64_t rs,
          const void* dy, int64_t dys, const void* w, int wtype,
-         const float* mean, const float* rstd, void* dx, void* dr, void* dw,
-         void* db, float* records, int n, int64_t rows, int H) {
+         const float* stats, void* dx, void* dr, void* dw, void* db,
+         float* records, int n, int64_t rows, int H) {
   if (group_of(H, kChunk<TX>) == 0) {
     if (dx || dr)
       hipLaunchKernelGGL((ln_bwd_long_kernel<TX, TR, TY, RES>),
                          dim3(at_most(rows, kMaxBlocks)), dim3(kLongThreads),
                          0, st, (const TX*)x, xs, (const TR*)r, rs,
-                         (const TY*)dy, dys, w, wtype, mean, rstd, (TX*)dx,
+                         (const TY*)dy, dys, w, wtype, stats, (TX*)dx,
                          (TR*)dr, rows, H);
     if (records)
       hipLaunchKernelGGL((ln_dw_long_kernel<TX, TR, TY, RES>),
                          dim3(n, at_most((H + 63) / 64, 65535)), dim3(256), 0,
                          st, (const TX*)x, xs, (const TR*)r, rs, (const TY*)dy,
-                         dys, mean, rstd, records, rows, H);
+                         dys, stats, records, rows, H);
   } else {
     with_group<kChunk<TX>>(H, [&](auto g, auto nv) {
       constexpr int G = decltype(g)::value, NV = decltype(nv)::value;
       constexpr int NT = G > 512 ? G : G > 64 ? 256 : 512;
       hipLaunchKernelGGL((ln_bwd_kernel<TX, TR, TY, RES, G, NV>), dim3(n),
                          dim3(NT), 0, st, (const TX*)x, xs, (const TR*)r, rs,
-                         (const TY*)dy, dys, w, wtype, mean, rstd, (TX*)dx,
+                         (const TY*)dy, dys, w, wtype, stats, (TX*)dx,
                          (TR*)dr, records, rows, H);
     });
   }
@@ -567,11 +616,10 @@ int64_t dear_ln_blocks(int xtype, int64_t rows, int H) {
 
 int dear_ln_fwd(hipStream_t st, int xtype, int rtype, int wtype, const void* x,
                 int64_t xs, const void* r, int64_t rs, const void* w,
-                const void* b, void* y, float* mean, float* rstd, int64_t rows,
-                int H, float eps) {
+                const void* b, void* y, float* stats, int64_t rows, int H,
+                float eps) {
 #define CALL(TX, TR, TY, RES)                                                 \
-  fwd<TX, TR, TY, RES>(st, x, xs, r, rs, w, b, wtype, y, mean, rstd, rows, H, \
-                       eps)
+  fwd<TX, TR, TY, RES>(st, x, xs, r, rs, w, b, wtype, y, stats, rows, H, eps)
   LN_DISPATCH(CALL);
 #undef CALL
   return (int)hipGetLastError();
@@ -580,12 +628,12 @@ int dear_ln_fwd(hipStream_t st, int xtype, int rtype, int wtype, const void* x,
 // records: n times 2 H floats, or null where neither dw nor db is wanted.
 int dear_ln_bwd(hipStream_t st, int xtype, int rtype, int wtype, const void* x,
                 int64_t xs, const void* r, int64_t rs, const void* dy,
-                int64_t dys, const void* w, const float* mean,
-                const float* rstd, void* dx, void* dr, void* dw, void* db,
-                float* records, int n, int64_t rows, int H) {
+                int64_t dys, const void* w, const float* stats, void* dx,
+                void* dr, void* dw, void* db, float* records, int n,
+                int64_t rows, int H) {
 #define CALL(TX, TR, TY, RES)                                                 \
-  bwd<TX, TR, TY, RES>(st, x, xs, r, rs, dy, dys, w, wtype, mean, rstd, dx,   \
-                       dr, dw, db, records, n, rows, H)
+  bwd<TX, TR, TY, RES>(st, x, xs, r, rs, dy, dys, w, wtype, stats, dx, dr,    \
+                       dw, db, records, n, rows, H)
   LN_DISPATCH(CALL);
 #undef CALL
   return (int)hipGetLastError();

@@ -11,12 +11,11 @@
 
 int64_t dear_ln_blocks(int, int64_t, int);
 int dear_ln_fwd(hipStream_t, int, int, int, const void*, int64_t, const void*,
-                int64_t, const void*, const void*, void*, float*, float*,
-                int64_t, int, float);
+                int64_t, const void*, const void*, void*, float*, int64_t, int,
+                float);
 int dear_ln_bwd(hipStream_t, int, int, int, const void*, int64_t, const void*,
                 int64_t, const void*, int64_t, const void*, const float*,
-                const float*, void*, void*, void*, void*, float*, int, int64_t,
-                int);
+                void*, void*, void*, void*, float*, int, int64_t, int);
 int64_t dear_logprobs_work(int, int64_t, int, int);
 int64_t dear_distill_work(int, int64_t, int);
 int dear_logprobs_fwd(hipStream_t, int, const void*, int64_t, const int64_t*,
@@ -137,18 +136,17 @@ Tensor ln_forward(const Tensor& x, const Tensor& w, const Tensor& b,
   const Tensor& wide = res.defined() ? res : x;
   Tensor y = at::empty(x.sizes(), wide.options());
   if (stats)
-    *stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
+    *stats = at::empty({3, rows}, x.options().dtype(at::kFloat));
   if (rows == 0) return y;
   const Tensor xr = as_rows(x, rows, width);
   const Tensor rr = res.defined() ? as_rows(res, rows, width) : Tensor();
   const Tensor& affine = w.defined() ? w : b;
-  float* mean = stats ? fdata(*stats) : nullptr;
   check_launch(dear_ln_fwd(
       stream_of(x), type_code(x, "x"),
       res.defined() ? type_code(res, "residual") : -1,
       affine.defined() ? type_code(affine, "weight") : 0, data(xr),
       xr.stride(0), data(rr), res.defined() ? rr.stride(0) : 0, data(w),
-      data(b), data(y), mean, mean ? mean + rows : nullptr, rows, (int)width,
+      data(b), data(y), stats ? fdata(*stats) : nullptr, rows, (int)width,
       (float)eps));
   return y;
 }
@@ -205,9 +203,8 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
           res.defined() ? type_code(res, "residual") : -1,
           affine.defined() ? type_code(affine, "weight") : 0, data(xr),
           xr.stride(0), data(rr), res.defined() ? rr.stride(0) : 0, data(gr),
-          gr.stride(0), data(w), fdata(stats), fdata(stats) + rows, data(dx),
-          data(dr), data(dw), data(db), fdata(part), (int)blocks, rows,
-          (int)width));
+          gr.stride(0), data(w), fdata(stats), data(dx), data(dr), data(dw),
+          data(db), fdata(part), (int)blocks, rows, (int)width));
     }
     return once({dx, dw, db, same ? dx : dr, Tensor()}, "layer_norm");
   }
