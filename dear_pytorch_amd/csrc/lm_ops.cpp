@@ -65,6 +65,17 @@ int64_t* idata(const Tensor& t) {
 using Maybe = c10::optional<Tensor>;
 Tensor value(const Maybe& t) { return t ? *t : Tensor(); }
 
+// What torch would see of an operand and the kernels do not: to go on would
+// lose it without a word.
+void check_operands(std::initializer_list<Tensor> ts, const char* name) {
+  for (const auto& t : ts) {
+    if (!t.defined()) continue;
+    TORCH_CHECK_NOT_IMPLEMENTED(
+        !t._fw_grad(/*level=*/0).defined(), name,
+        ": forward-mode derivatives are not there on a GPU");
+  }
+}
+
 hipStream_t stream_of(const Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
@@ -170,6 +181,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
                  &stats = saved[3];
     const Tensor& affine = w.defined() ? w : saved[4];
     const c10::DeviceGuard guard(x.device());
+    check_operands({up[0]}, "layer_norm");
     check_capture({x, affine, res}, stream_of(x), "layer_norm");
     const auto [rows, width] = ln_shape(x);
     // the node has an edge for each tensor that was given
@@ -215,6 +227,7 @@ Tensor layer_norm(const Tensor& x, const Maybe& weight,
                   const Maybe& residual) {
   Tensor a = x, r = value(residual);
   const Tensor w = value(weight), b = value(bias);
+  check_operands({x, r, w, b}, "layer_norm");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) < kMaxWidth,
                     "layer_norm: x needs a last axis of 1 to 2^30 - 1 "
                     "elements");
@@ -337,6 +350,7 @@ struct LogprobsFn : torch::autograd::Function<LogprobsFn> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &tokens = saved[1];
     const c10::DeviceGuard guard(logits.device());
+    for (const auto& u : up) check_operands({u}, "token_logprobs");
     check_capture({logits}, stream_of(logits), "token_logprobs");
     const int64_t top = ctx->saved_data["top"].toInt();
     const size_t at0 = tokens.defined() ? 1 : 0;
@@ -365,6 +379,7 @@ variable_list token_logprobs(const Tensor& logits,
                              const Maybe& tokens_, int64_t top,
                              double t, int64_t ignore) {
   const Tensor tokens = value(tokens_);
+  check_operands({logits}, "token_logprobs");
   check_logits(logits, "token_logprobs");
   TORCH_CHECK_VALUE(top >= 0 && top <= kMaxTop && top <= logits.size(-1),
                     "token_logprobs: top must be 0 to ", kMaxTop,
@@ -426,6 +441,7 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &ids = saved[1];
     const c10::DeviceGuard guard(logits.device());
+    check_operands({up[0]}, "topk_distill_loss");
     check_capture({logits}, stream_of(logits), "topk_distill_loss");
     const auto z = logit_rows(logits);
     Tensor dz = at::empty(logits.sizes(), logits.options());
@@ -445,6 +461,7 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
 
 Tensor topk_distill_loss(const Tensor& logits, const Tensor& ids,
                          const Tensor& teacher, double t, bool tail) {
+  check_operands({logits, teacher}, "topk_distill_loss");
   check_logits(logits, "topk_distill_loss");
   type_code(teacher, "top_logprobs");
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);

@@ -1,0 +1,92 @@
+"""What the language-model operators' kernels cannot see of an operand, and so
+refuse: a tangent. The refusals are in front of every look at the device, so
+that they can be tested without one."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+
+from dear_pytorch_amd.ops.fused_ln import layer_norm
+from dear_pytorch_amd.ops.token_loss import token_logprobs, topk_distill_loss
+
+
+def operands(dev, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(3, 8, generator=gen)
+    ids = torch.tensor([[1, 2], [3, 4], [0, 7]])
+    lp = torch.log_softmax(torch.randn(3, 8, generator=gen), -1).gather(1, ids)
+    w = torch.randn(8, generator=gen)
+    return {k: t.to(dev) for k, t in
+            dict(x=x, w=w, b=w - 1, r=x.flip(0), ids=ids, lp=lp).items()}
+
+
+# the public entry points, and the operands of each that are numbers
+CALLS = {
+    "layer_norm": (lambda o: layer_norm(o["x"], o["w"], o["b"], 1e-5,
+                                        residual=o["r"]),
+                   ("x", "w", "b", "r")),
+    "token_logprobs": (lambda o: token_logprobs(o["x"], o["ids"][:, 0],
+                                                top=2).logprob, ("x",)),
+    "topk_distill_loss": (lambda o: topk_distill_loss(o["x"], o["ids"],
+                                                      o["lp"], tail=True),
+                          ("x", "lp")),
+}
+
+
+# the same calls of the extension, which refuses before it asks for the device
+def native(name):
+    k = pytest.importorskip("dear_pytorch_amd._kernels")
+    return {
+        "layer_norm": lambda o: k.layer_norm(o["x"], o["w"], o["b"], 1e-5,
+                                             o["r"]),
+        "token_logprobs": lambda o: k.token_logprobs(
+            o["x"], o["ids"][:, 0].contiguous(), 2, 1.0, -1),
+        "topk_distill_loss": lambda o: k.topk_distill_loss(
+            o["x"], o["ids"], o["lp"], 1.0, True),
+    }[name]
+
+
+EACH = [(n, k) for n, (_, keys) in CALLS.items() for k in keys]
+
+
+def tangents(call, name, key, dev):
+    for grad in (False, True):
+        o = operands(dev)
+        if grad:
+            o["x"].requires_grad_(True)
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), fw.dual_level():
+                dual = dict(o)
+                dual[key] = fw.make_dual(o[key], torch.ones_like(o[key]))
+                with pytest.raises(NotImplementedError, match=name):
+                    call(dual)
+
+
+@pytest.mark.parametrize("name,key", EACH)
+def test_tangents_are_refused(name, key):
+    tangents(native(name), name, key, "cpu")
+
+
+def test_cpu_paths_have_tangents():
+    for name, (call, keys) in CALLS.items():
+        o = operands("cpu")
+        with fw.dual_level():
+            o["x"] = fw.make_dual(o["x"], torch.ones_like(o["x"]) * 0.3)
+            assert fw.unpack_dual(call(o)).tangent is not None, name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,key", EACH)
+def test_gpu_tangents_are_refused(name, key):
+    tangents(CALLS[name][0], name, key, "cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", CALLS)
+def test_gpu_tangents_of_upstream_gradients_are_refused(name):
+    o = operands("cuda")
+    o["x"].requires_grad_(True)
+    y = CALLS[name][0](o)
+    with fw.dual_level():
+        up = fw.make_dual(torch.ones_like(y), torch.ones_like(y))
+        with pytest.raises(NotImplementedError, match=name):
+            torch.autograd.grad(y, o["x"], up)
