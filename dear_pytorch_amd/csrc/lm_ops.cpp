@@ -3,11 +3,13 @@
 // token or a small batch the host's work, not the kernel, is the cost.
 #include <torch/extension.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 int64_t dear_ln_blocks(int, int64_t, int);
 int dear_ln_fwd(hipStream_t, int, int, int, const void*, int64_t, const void*,
@@ -68,6 +70,13 @@ Tensor value(const Maybe& t) { return t ? *t : Tensor(); }
 // What torch would see of an operand and the kernels do not: to go on would
 // lose it without a word.
 void check_operands(std::initializer_list<Tensor> ts, const char* name) {
+  // a trace would hold the results' allocation, and nothing that fills them
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !torch::jit::tracer::isTracing() &&
+          !c10::impl::TorchDispatchModeTLS::get_mode(
+               c10::impl::TorchDispatchModeKey::PROXY)
+               .has_value(),
+      name, ": cannot be traced on a GPU");
   for (const auto& t : ts) {
     if (!t.defined()) continue;
     TORCH_CHECK_NOT_IMPLEMENTED(

@@ -16,7 +16,8 @@ gradients of x and residual are the same numbers, and the same tensor where
 they have the same type. It is differentiable once.
 
 On the CPU the same numbers come from a torch composition; on a GPU the native
-extension is required, and forward-mode derivatives raise.
+extension is required, and forward-mode derivatives and tracing
+(torch.jit.trace, make_fx) raise.
 """
 from __future__ import annotations
 

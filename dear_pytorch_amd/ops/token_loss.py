@@ -13,7 +13,8 @@ last; results are float32. A row whose logits hold NaN or +inf, or nothing but
 id outside of the vocabulary gives NaN as well, and nothing is read there.
 
 On the CPU the same numbers come from a torch composition; on a GPU the native
-extension is required, and forward-mode derivatives raise.
+extension is required, and forward-mode derivatives and tracing
+(torch.jit.trace, make_fx) raise.
 """
 from __future__ import annotations
 

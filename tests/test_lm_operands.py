@@ -1,9 +1,10 @@
 """What the language-model operators' kernels cannot see of an operand, and so
-refuse: a tangent. The refusals are in front of every look at the device, so
+refuse: a tangent, a tracer. The refusals are in front of every look at the device, so
 that they can be tested without one."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from dear_pytorch_amd.ops.fused_ln import layer_norm
 from dear_pytorch_amd.ops.token_loss import token_logprobs, topk_distill_loss
@@ -72,6 +73,38 @@ def test_cpu_paths_have_tangents():
         with fw.dual_level():
             o["x"] = fw.make_dual(o["x"], torch.ones_like(o["x"]) * 0.3)
             assert fw.unpack_dual(call(o)).tangent is not None, name
+
+
+def traces(call, name, dev):
+    o = operands(dev)
+    for grad in (False, True):
+        x = o["x"].clone().requires_grad_(grad)
+        with pytest.raises(NotImplementedError, match=name):
+            torch.jit.trace(lambda x: call({**o, "x": x}), (x,))
+        with pytest.raises(NotImplementedError, match=name):
+            make_fx(lambda x: call({**o, "x": x}))(x)
+    assert not torch.jit.is_tracing()
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_tracing_is_refused(name):
+    traces(native(name), name, "cpu")
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_cpu_paths_can_be_traced(name):
+    o, call = operands("cpu"), CALLS[name][0]
+    run = lambda x: call({**o, "x": x})
+    for traced in (torch.jit.trace(run, (o["x"],), check_trace=False),
+                   make_fx(run)(o["x"])):
+        x = operands("cpu", seed=1)["x"]
+        assert torch.equal(traced(x), run(x))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", CALLS)
+def test_gpu_tracing_is_refused(name):
+    traces(CALLS[name][0], name, "cuda")
 
 
 @pytest.mark.gpu
