@@ -7,8 +7,9 @@
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
-#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 int64_t dear_ln_blocks(int, int64_t, int);
@@ -108,28 +109,29 @@ variable_list once(variable_list grads, const char* name) {
   return (*node)(std::move(grads));
 }
 
-// Whether a leaf's gradient is accumulated on another stream than the current
-// one, as it is while a graph that was made there lives.
-bool accumulates_elsewhere(const Tensor& leaf) {
-  if (!leaf.defined() || !leaf.requires_grad() || !leaf.is_leaf()) return false;
-  const auto node = torch::autograd::impl::try_get_grad_accumulator(leaf);
-  const auto stream = node ? node->stream() : std::nullopt;
-  const c10::impl::VirtualGuardImpl guard(leaf.device().type());
-  return stream && *stream != guard.getStream(leaf.device());
+// Whether a node adds up a leaf's gradient on another stream than the current
+// one, as it does while a graph that was made there lives.
+bool accumulates_elsewhere(torch::autograd::Node* node) {
+  if (!dynamic_cast<torch::autograd::AccumulateGrad*>(node)) return false;
+  const auto stream = node->stream();
+  if (!stream) return false;
+  const c10::impl::VirtualGuardImpl guard(stream->device_type());
+  return *stream != guard.getStream(stream->device());
 }
 
 // A captured backward pass cannot hand a gradient to a stream outside of the
-// capture; the process would end where it tries to.
-void check_capture(std::initializer_list<Tensor> leaves, hipStream_t stream,
-                   const char* name) {
+// capture; the process would end where it tries to. To be called in a node's
+// backward pass: looks at the leaves behind it.
+void check_capture(hipStream_t stream, const char* name) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   check_launch((int)hipStreamIsCapturing(stream, &status));
   if (status == hipStreamCaptureStatusNone) return;
-  for (const auto& t : leaves)
-    TORCH_CHECK(!accumulates_elsewhere(t), name, ": a backward pass is being "
-                "captured while a graph of the same leaf that was made on "
-                "another stream is alive; free that one first, or make it on "
-                "the stream of the capture");
+  const auto node = torch::autograd::get_current_node();
+  for (size_t i = 0; node && i < node->num_outputs(); ++i)
+    TORCH_CHECK(!accumulates_elsewhere(node->next_edge(i).function.get()), name,
+                ": a backward pass is being captured while a graph of the same "
+                "leaf that was made on another stream is alive; free that one "
+                "first, or make it on the stream of the capture");
 }
 
 bool wants_grad(std::initializer_list<Tensor> ts) {
@@ -191,7 +193,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     const Tensor& affine = w.defined() ? w : saved[4];
     const c10::DeviceGuard guard(x.device());
     check_operands({up[0]}, "layer_norm");
-    check_capture({x, affine, res}, stream_of(x), "layer_norm");
+    check_capture(stream_of(x), "layer_norm");
     const auto [rows, width] = ln_shape(x);
     // the node has an edge for each tensor that was given
     const bool has_b = ctx->saved_data["bias"].toBool();
@@ -360,7 +362,7 @@ struct LogprobsFn : torch::autograd::Function<LogprobsFn> {
     const Tensor &logits = saved[0], &tokens = saved[1];
     const c10::DeviceGuard guard(logits.device());
     for (const auto& u : up) check_operands({u}, "token_logprobs");
-    check_capture({logits}, stream_of(logits), "token_logprobs");
+    check_capture(stream_of(logits), "token_logprobs");
     const int64_t top = ctx->saved_data["top"].toInt();
     const size_t at0 = tokens.defined() ? 1 : 0;
     const Tensor dlp = tokens.defined() ? up_of(up, 0) : Tensor();
@@ -451,7 +453,7 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
     const Tensor &logits = saved[0], &ids = saved[1];
     const c10::DeviceGuard guard(logits.device());
     check_operands({up[0]}, "topk_distill_loss");
-    check_capture({logits}, stream_of(logits), "topk_distill_loss");
+    check_capture(stream_of(logits), "topk_distill_loss");
     const auto z = logit_rows(logits);
     Tensor dz = at::empty(logits.sizes(), logits.options());
     if (z.rows) {
