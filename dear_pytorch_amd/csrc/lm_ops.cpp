@@ -121,17 +121,19 @@ bool accumulates_elsewhere(torch::autograd::Node* node) {
 
 // A captured backward pass cannot hand a gradient to a stream outside of the
 // capture; the process would end where it tries to. To be called in a node's
-// backward pass: looks at the leaves behind it.
+// backward pass: looks at the leaves behind it that this pass has a gradient
+// for.
 void check_capture(hipStream_t stream, const char* name) {
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   check_launch((int)hipStreamIsCapturing(stream, &status));
   if (status == hipStreamCaptureStatusNone) return;
   const auto node = torch::autograd::get_current_node();
   for (size_t i = 0; node && i < node->num_outputs(); ++i)
-    TORCH_CHECK(!accumulates_elsewhere(node->next_edge(i).function.get()), name,
-                ": a backward pass is being captured while a graph of the same "
-                "leaf that was made on another stream is alive; free that one "
-                "first, or make it on the stream of the capture");
+    TORCH_CHECK(!node->task_should_compute_output(i) ||
+                    !accumulates_elsewhere(node->next_edge(i).function.get()),
+                name, ": a backward pass is being captured while a graph of "
+                "the same leaf that was made on another stream is alive; free "
+                "that one first, or make it on the stream of the capture");
 }
 
 bool wants_grad(std::initializer_list<Tensor> ts) {

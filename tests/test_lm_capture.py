@@ -66,3 +66,15 @@ def test_gpu_the_bias_alone_lives_elsewhere():
     want = torch.autograd.grad(call(t), t, up)
     graph, got = captured(lambda: torch.autograd.grad(call(t), t, up))
     replayed(graph, got, want)
+
+
+@pytest.mark.gpu
+def test_gpu_a_leaf_that_nothing_is_asked_of_may_live_elsewhere():
+    t = [v.requires_grad_(True) for v in leaves()]
+    up = torch.ones(6, 64, device="cuda")
+    want = torch.autograd.grad(call(t), t, up)
+    other = t[1] * 2.0 + t[2]             # eager graphs of weight and bias
+    asked = [t[0], t[3]]
+    graph, got = captured(lambda: torch.autograd.grad(call(t), asked, up))
+    replayed(graph, got, [want[0], want[3]])
+    del other
