@@ -83,6 +83,9 @@ void check_operands(std::initializer_list<Tensor> ts, const char* name) {
     TORCH_CHECK_NOT_IMPLEMENTED(
         !t._fw_grad(/*level=*/0).defined(), name,
         ": forward-mode derivatives are not there on a GPU");
+    // wrappers of other tensors, and fake ones
+    TORCH_CHECK_TYPE(t.numel() == 0 || t.const_data_ptr() != nullptr, name,
+                     ": an operand has no memory of its own");
   }
 }
 
@@ -392,7 +395,7 @@ variable_list token_logprobs(const Tensor& logits,
                              const Maybe& tokens_, int64_t top,
                              double t, int64_t ignore) {
   const Tensor tokens = value(tokens_);
-  check_operands({logits}, "token_logprobs");
+  check_operands({logits, tokens}, "token_logprobs");
   check_logits(logits, "token_logprobs");
   TORCH_CHECK_VALUE(top >= 0 && top <= kMaxTop && top <= logits.size(-1),
                     "token_logprobs: top must be 0 to ", kMaxTop,
@@ -474,7 +477,7 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
 
 Tensor topk_distill_loss(const Tensor& logits, const Tensor& ids,
                          const Tensor& teacher, double t, bool tail) {
-  check_operands({logits, teacher}, "topk_distill_loss");
+  check_operands({logits, ids, teacher}, "topk_distill_loss");
   check_logits(logits, "topk_distill_loss");
   type_code(teacher, "top_logprobs");
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);

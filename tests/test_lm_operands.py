@@ -1,9 +1,10 @@
 """What the language-model operators' kernels cannot see of an operand, and so
-refuse: a tangent, a tracer. The refusals are in front of every look at the device, so
+refuse: a tangent, a tracer, another tensor inside. The refusals are in front of every look at the device, so
 that they can be tested without one."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
+from torch._subclasses import FakeTensorMode
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from dear_pytorch_amd.ops.fused_ln import layer_norm
@@ -99,6 +100,45 @@ def test_cpu_paths_can_be_traced(name):
                    make_fx(run)(o["x"])):
         x = operands("cpu", seed=1)["x"]
         assert torch.equal(traced(x), run(x))
+
+
+class Wrapper(torch.Tensor):
+    """A tensor around another one, as distributed tensors are."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(
+            cls, t.shape, dtype=t.dtype, device=t.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError(func)
+
+
+EVERY = [(n, k) for n, keys in (
+    ("layer_norm", ("x", "w", "b", "r")), ("token_logprobs", ("x", "tokens")),
+    ("topk_distill_loss", ("x", "ids", "lp"))) for k in keys]
+
+
+@pytest.mark.parametrize("name,key", EVERY)
+def test_operands_without_memory_are_refused(name, key):
+    k = pytest.importorskip("dear_pytorch_amd._kernels")
+    call = native(name)
+    if key == "tokens":
+        call = lambda o: k.token_logprobs(o["x"], o["tokens"], 2, 1.0, -1)
+    with FakeTensorMode():
+        fake = operands("cpu")
+        fake["tokens"] = torch.zeros(3, dtype=torch.long)
+    for grad in (False, True):
+        o = operands("cpu")
+        o["tokens"] = o["ids"][:, 0].contiguous()
+        if key != "x":
+            o["x"].requires_grad_(grad)
+        for bad in (Wrapper(o[key]), fake[key],
+                    torch._efficientzerotensor(o[key].shape,
+                                               dtype=o[key].dtype)):
+            with pytest.raises(TypeError, match=name):
+                call({**o, key: bad})
 
 
 @pytest.mark.gpu
