@@ -68,6 +68,12 @@ int64_t* idata(const Tensor& t) {
 using Maybe = c10::optional<Tensor>;
 Tensor value(const Maybe& t) { return t ? *t : Tensor(); }
 
+// A view whose elements are to be negated when they are read, as the imaginary
+// part of a conjugate is: the kernels do not do that.
+Tensor plain(const Tensor& t) {
+  return t.defined() && t.is_neg() ? t.resolve_neg() : t;
+}
+
 // What torch would see of an operand and the kernels do not: to go on would
 // lose it without a word.
 void check_operands(std::initializer_list<Tensor> ts, const char* name) {
@@ -221,7 +227,7 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
     } else {
       const Tensor xr = as_rows(x, rows, width);
       const Tensor rr = res.defined() ? as_rows(res, rows, width) : Tensor();
-      const Tensor gr = as_rows(up[0], rows, width);
+      const Tensor gr = as_rows(plain(up[0]), rows, width);
       const int64_t blocks = dear_ln_blocks(type_code(x, "x"), rows,
                                             (int)width);
       if (want_w || want_b)
@@ -241,9 +247,9 @@ struct LayerNormFn : torch::autograd::Function<LayerNormFn> {
 Tensor layer_norm(const Tensor& x, const Maybe& weight,
                   const Maybe& bias, double eps,
                   const Maybe& residual) {
-  Tensor a = x, r = value(residual);
-  const Tensor w = value(weight), b = value(bias);
-  check_operands({x, r, w, b}, "layer_norm");
+  Tensor a = plain(x), r = plain(value(residual));
+  Tensor w = value(weight), b = value(bias);
+  check_operands({a, r, w, b}, "layer_norm");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) < kMaxWidth,
                     "layer_norm: x needs a last axis of 1 to 2^30 - 1 "
                     "elements");
@@ -275,6 +281,8 @@ Tensor layer_norm(const Tensor& x, const Maybe& weight,
                        w.scalar_type() == b.scalar_type(),
                    "layer_norm: weight and bias are of two types");
   TORCH_CHECK_VALUE(x.is_cuda(), "layer_norm: x is not on a GPU");
+  w = plain(w);
+  b = plain(b);
   if (!wants_grad({a, w, b, r})) return ln_forward(a, w, b, r, eps, nullptr);
   return LayerNormFn::apply(a, maybe(w), maybe(b), maybe(r), eps);
 }
@@ -343,7 +351,7 @@ variable_list logprobs_forward(const Tensor& logits, const Tensor& tokens,
 }
 
 Tensor up_of(const variable_list& up, size_t i) {
-  return up[i].defined() ? up[i].contiguous() : Tensor();
+  return up[i].defined() ? plain(up[i]).contiguous() : Tensor();
 }
 
 struct LogprobsFn : torch::autograd::Function<LogprobsFn> {
@@ -391,10 +399,9 @@ struct LogprobsFn : torch::autograd::Function<LogprobsFn> {
   }
 };
 
-variable_list token_logprobs(const Tensor& logits,
-                             const Maybe& tokens_, int64_t top,
-                             double t, int64_t ignore) {
-  const Tensor tokens = value(tokens_);
+variable_list token_logprobs(const Tensor& logits_, const Maybe& tokens_,
+                             int64_t top, double t, int64_t ignore) {
+  const Tensor logits = plain(logits_), tokens = plain(value(tokens_));
   check_operands({logits, tokens}, "token_logprobs");
   check_logits(logits, "token_logprobs");
   TORCH_CHECK_VALUE(top >= 0 && top <= kMaxTop && top <= logits.size(-1),
@@ -462,7 +469,7 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
     const auto z = logit_rows(logits);
     Tensor dz = at::empty(logits.sizes(), logits.options());
     if (z.rows) {
-      const Tensor idc = ids.contiguous(), g = up[0].contiguous();
+      const Tensor idc = ids.contiguous(), g = up_of(up, 0);
       check_launch(dear_distill_bwd(
           stream_of(logits), type_code(logits, "logits"), data(z.t),
           z.t.dim() == 2 ? z.t.stride(0) : 0, idata(idc),
@@ -475,8 +482,10 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
   }
 };
 
-Tensor topk_distill_loss(const Tensor& logits, const Tensor& ids,
-                         const Tensor& teacher, double t, bool tail) {
+Tensor topk_distill_loss(const Tensor& logits_, const Tensor& ids_,
+                         const Tensor& teacher_, double t, bool tail) {
+  const Tensor logits = plain(logits_), ids = plain(ids_),
+               teacher = plain(teacher_);
   check_operands({logits, ids, teacher}, "topk_distill_loss");
   check_logits(logits, "topk_distill_loss");
   type_code(teacher, "top_logprobs");

@@ -1,6 +1,6 @@
-"""What the language-model operators' kernels cannot see of an operand, and so
-refuse: a tangent, a tracer, another tensor inside. The refusals are in front of every look at the device, so
-that they can be tested without one."""
+"""What the language-model operators' kernels cannot see of an operand: a tangent,
+a tracer and another tensor inside are refused, in front of every look at the
+device, so that this can be tested without one; a negation is resolved."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
@@ -163,3 +163,25 @@ def test_gpu_tangents_of_upstream_gradients_are_refused(name):
         up = fw.make_dual(torch.ones_like(y), torch.ones_like(y))
         with pytest.raises(NotImplementedError, match=name):
             torch.autograd.grad(y, o["x"], up)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,key", EACH)
+def test_gpu_operands_that_are_negated_when_read(name, key):
+    """The same numbers as their copies, upstream gradients as well."""
+    def both(o, change):
+        o["x"] = o["x"].detach().requires_grad_(True)
+        y = call({**o, key: change(o[key])})
+        with torch.no_grad():
+            again = call({**o, key: change(o[key])})
+        up = change(torch.full_like(y, 0.75))
+        return y.detach(), again, torch.autograd.grad(y, o["x"], up)[0]
+
+    def negated(t):
+        t = torch._neg_view(-t)
+        assert t.is_neg() and t.is_contiguous()
+        return t
+
+    call, o = CALLS[name][0], operands("cuda")
+    want, got = both(o, lambda t: t), both(o, negated)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
