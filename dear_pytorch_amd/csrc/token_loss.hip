@@ -1071,7 +1071,8 @@ __global__ __launch_bounds__(kBwdThreads) void logprobs_bwd_kernel(
       const float y = (v - s.m) * c;
       const float e = __builtin_amdgcn_exp2f(y) * scale;
       if constexpr (ENT)
-        return e * fmaf(dh, fmaf(fmaxf(y, -1e30f), (float)kLn2, s.a), a);
+        // e is 0 from -150 on: no product with it may be infinite
+        return e * fmaf(dh, fmaf(fmaxf(y, -256.f), (float)kLn2, s.a), a);
       return e * a;
     };
     map_piece<STREAM>(z, out, len, spread);
