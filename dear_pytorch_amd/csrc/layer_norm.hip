@@ -375,18 +375,24 @@ __global__ __launch_bounds__(1024) void ln_records_kernel(
     void* __restrict__ db, int wtype) {
   __shared__ float part[16][64];
   const int lane = threadIdx.x & 63, sub = threadIdx.x >> 6;
-  const int64_t i = (int64_t)blockIdx.x * 64 + lane;
-  float s = 0.f;
-  if (i < 2 * (int64_t)H) {
+  const int64_t columns = 2 * (int64_t)H;
+  for (int64_t first = (int64_t)blockIdx.x * 64; first < columns;
+       first += (int64_t)gridDim.x * 64) {
+    const int64_t i = first + lane;
+    float s = 0.f;
+    if (i < columns) {
 #pragma unroll 8
-    for (int k = sub; k < n; k += 16) s += records[(int64_t)k * 2 * H + i];
+      for (int k = sub; k < n; k += 16) s += records[k * columns + i];
+    }
+    part[sub][lane] = s;
+    __syncthreads();
+    if (sub == 0 && i < columns) {
+      for (int k = 1; k < 16; ++k) s += part[k][lane];
+      void* out = i < H ? dw : db;
+      if (out) store_as(out, wtype, i < H ? i : i - H, s);
+    }
+    __syncthreads();                     // before `part` is written again
   }
-  part[sub][lane] = s;
-  __syncthreads();
-  if (sub != 0 || i >= 2 * (int64_t)H) return;
-  for (int k = 1; k < 16; ++k) s += part[k][lane];
-  void* out = i < H ? dw : db;
-  if (out) store_as(out, wtype, i < H ? i : i - H, s);
 }
 
 // ------------------------------------------------------------- long rows
@@ -589,7 +595,8 @@ void bwd(hipStream_t st, const void* x, int64_t xs, const void* r, int64_t rs,
     });
   }
   if (records)
-    hipLaunchKernelGGL(ln_records_kernel, dim3((2 * (int64_t)H + 63) / 64),
+    hipLaunchKernelGGL(ln_records_kernel,
+                       dim3(at_most((2 * (int64_t)H + 63) / 64, kMaxBlocks)),
                        dim3(1024), 0, st, records, n, H, dw, db, wtype);
 }
 

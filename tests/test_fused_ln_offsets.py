@@ -131,3 +131,20 @@ def test_gpu_rows_of_both_kinds_share_a_wave():
         x[::3] = x[::3, :1]                      # no spread
         x[1::4] += 1000.1
         compare(x, 1e-12)
+
+
+@pytest.mark.gpu
+def test_gpu_wider_than_a_launch_of_its_columns():
+    """Over 2^27 columns: their sums of 1024 threads for 64 of them would be
+    more threads than a launch holds."""
+    H = (1 << 27) + 70
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x, dy = torch.randn(2, 1, H, generator=gen, device="cuda")
+    w, b = torch.ones(H, device="cuda"), torch.zeros(H, device="cuda")
+    _, g = run(x, w, b, 1e-5, None, dy)
+    assert torch.equal(g["b"], dy[0])
+    z = x[0].double()
+    n = (z - z.mean()) / (z.var(correction=0) + 1e-5).sqrt()
+    # n rounds in a difference of three, a root, a quotient and a product
+    err = 8 * U * (n.abs() + 1)
+    check(g["w"], (dy[0] * n, dy[0].abs().double() * err), "w")
