@@ -396,6 +396,8 @@ __global__ __launch_bounds__(1024) void ln_records_kernel(
 }
 
 // ------------------------------------------------------------- long rows
+// A thread adds up a thousandth of the row: in fp64, for a chain of that many
+// float32 additions would be as far off as its length.
 constexpr int kLongThreads = 1024;
 
 template <typename TX, typename TR, bool RES>
@@ -445,21 +447,21 @@ __global__ __launch_bounds__(kLongThreads) void ln_bwd_long_kernel(
     const TY* __restrict__ dy, int64_t dys, const void* __restrict__ w,
     int wtype, const float* __restrict__ stats, TX* __restrict__ dx,
     TR* __restrict__ dr, int64_t rows, int H) {
-  __shared__ float scratch[kLongThreads / 64];
+  __shared__ double scratch[kLongThreads / 64];
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const TX* xr = x + row * xs;
     const TR* rr = RES ? r + row * rs : nullptr;
     const TY* gr = dy + row * dys;
     const RowNorm stat = get_stats(stats, rows, row);
-    float sg = 0.f, sgn = 0.f;
+    double all_g = 0.0, all_gn = 0.0;
     for (int i = threadIdx.x; i < H; i += kLongThreads) {
       float g = to_f(gr[i]);
       if (w) g *= load_as_float(w, wtype, i);
-      sg += g;
-      sgn += g * norm_of(load_z<TX, TR, RES>(xr, rr, i), stat);
+      all_g += g;
+      all_gn += g * norm_of(load_z<TX, TR, RES>(xr, rr, i), stat);
     }
-    sg = block_reduce(sg, Add{}, scratch) / (float)H;
-    sgn = block_reduce(sgn, Add{}, scratch) / (float)H;
+    const float sg = (float)(block_reduce(all_g, Add{}, scratch) / H);
+    const float sgn = (float)(block_reduce(all_gn, Add{}, scratch) / H);
     for (int i = threadIdx.x; i < H; i += kLongThreads) {
       float g = to_f(gr[i]);
       if (w) g *= load_as_float(w, wtype, i);

@@ -148,3 +148,27 @@ def test_gpu_wider_than_a_launch_of_its_columns():
     # n rounds in a difference of three, a root, a quotient and a product
     err = 8 * U * (n.abs() + 1)
     check(g["w"], (dy[0] * n, dy[0].abs().double() * err), "w")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [20011, 3000001])
+def test_gpu_long_rows_sum_without_drift(H):
+    """A constant upstream gradient, which each thread adds up in one chain: the
+    gradient of x is what the sums leave of it, and these are float64 here. The
+    products round once each, and g - mean g - n mean(g n) twice more."""
+    gen = torch.Generator().manual_seed(H)
+    x = torch.randn(2, H, generator=gen).cuda()
+    dy = torch.full_like(x, 0.1)
+    dy[1, ::2] = 0.3
+    _, g = run(x, None, None, 1e-5, None, dy)
+    z, up = x.double(), dy.double()
+    d = z - z.mean(-1, keepdim=True)
+    rstd = 1.0 / (d.square().mean(-1, keepdim=True) + 1e-5).sqrt()
+    n = d * rstd
+    mgn = (up * n).mean(-1, keepdim=True)
+    dz = rstd * (up - up.mean(-1, keepdim=True) - n * mgn)
+    # n is off by 8 u (|n| + 1); the mean of g n by as much of mean |g n|
+    off = (up.abs() * 8 * U * (n.abs() + 1)).mean(-1, keepdim=True)
+    err = rstd * (4 * U * up.abs() + off * n.abs()
+                  + 8 * U * (n.abs() + 1) * mgn.abs()) + 6 * U * dz.abs()
+    check(g["x"], (dz, err), "x")
