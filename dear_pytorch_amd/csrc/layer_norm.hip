@@ -187,6 +187,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 4) void ln_fwd_kernel(
   float wv[N], bv[N];
   load_columns<NV, E>(wv, w, wtype, first, G * E, H, 1.f);
   load_columns<NV, E>(bv, b, wtype, first, G * E, H, 0.f);
+  const float inv_h = 1.0f / (float)H;
   for (int64_t row = (int64_t)blockIdx.x * (NT / G) + threadIdx.x / G;
        row < rows; row += (int64_t)gridDim.x * (NT / G)) {
     Chunk<TX, E> cx[NV];
@@ -206,6 +207,8 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 4) void ln_fwd_kernel(
         z[c * E + j] = v;
         s += v;
       }
+    // a quotient: a product could be joined with the differences to it, which
+    // would then be to another number than this one
     float mean = group_sum(s) / (float)H, off = 0.f, q = 0.f;
     auto inside = [&](int c, int j) { return first + c * G * E + j < H; };
 #pragma unroll
@@ -219,9 +222,10 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 4) void ln_fwd_kernel(
       }
     group_sum(off, q);
     // the same in all threads of the group, which meet again in the sums
-    const bool again = 64.f * off * (off / (float)H) > q;
-    off /= (float)H;
-    float var = q / (float)H - off * off;
+    off *= inv_h;
+    q *= inv_h;
+    const bool again = 64.f * off * off > q;
+    float var = q - off * off;
     if (again) {
       const float better = mean + off, step = better - mean;
       mean = better;
@@ -233,7 +237,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 4) void ln_fwd_kernel(
           if (inside(c, j)) z[c * E + j] -= step;
           off += z[c * E + j];
         }
-      off = group_sum(off) / (float)H;
+      off = group_sum(off) * inv_h;
 #pragma unroll
       for (int c = 0; c < NV; ++c)
 #pragma unroll
@@ -241,7 +245,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 4) void ln_fwd_kernel(
           const float d = inside(c, j) ? z[c * E + j] - off : 0.f;
           q = fmaf(d, d, q);
         }
-      var = group_sum(q) / (float)H;
+      var = group_sum(q) * inv_h;
     }
     const float rstd = 1.0f / sqrtf(var + eps);
 #pragma unroll
