@@ -1,7 +1,7 @@
 // Layer norm over the last axis with an optional residual add, forward and
 // backward, for gfx950.
 //
-//   z = x + residual           (in fp32; never rounded, never stored)
+//   z = x + residual           (an fp32 sum; never stored)
 //   mean = sum(z) / H          rstd = 1 / sqrt(sum((z - mean)^2) / H + eps)
 //   n = (z - mean) * rstd      y = n * weight + bias
 // backward, with g = dy * weight:
@@ -167,13 +167,13 @@ __device__ __forceinline__ void load_columns(float (&v)[NV * E], const void* p,
   }
 }
 
-// Bound by memory: 16384 x 1024, a bf16 branch on an fp32 residual, takes 23 us
-// (7.3 TB/s, part of it from the last-level cache; 34 us where nothing of it is
-// there), 4096 x 768 fp32 5.9 us. One row takes 2.5 us, a launch's own time.
+// Bound by memory: 16384 x 1024, a bf16 branch on an fp32 residual, takes 26 us
+// (6.4 TB/s, part of it from the last-level cache; 34 us where nothing of it is
+// there), 4096 x 768 fp32 5.9 us. One row takes 2.2 us, a launch's own time.
 // 256 threads hold one to sixteen rows: a wave to a row of up to 1024 elements
 // needs no barrier, and the lanes' sums go through DPP, not LDS. Against one
 // block to a row with elements loaded one by one: 254 us for this pass and the
-// backward's, 83 now.
+// backward's, 84 now.
 template <typename TX, typename TR, typename TY, bool RES, int G, int NV>
 __global__ __launch_bounds__(G > 256 ? G : 256, 4) void ln_fwd_kernel(
     const TX* __restrict__ x, int64_t xs, const TR* __restrict__ r, int64_t rs,
@@ -261,12 +261,11 @@ __global__ __launch_bounds__(G > 256 ? G : 256, 4) void ln_fwd_kernel(
   }
 }
 
-// Bound by memory as well: the same case takes 46 us (5.9 TB/s; 56 us where
-// nothing is cached), 4096 x 768 fp32 14 us. Few blocks, each of many rows, as
-// many as leave 256 records: a record per row would be as many bytes again as
-// the gradient. Gradients that are stored past the caches are written no
-// faster here (93 us for a pass instead of 83): what reads them next then has
-// to fetch them.
+// Bound by memory as well: the same case takes 47 us (5.8 TB/s); 4096 x 768
+// fp32, 12.7 us, by its few waves. Few blocks, each of many rows, as many as
+// leave 256 records: a record per row would be as many bytes again as the
+// gradient. Gradients that are stored past the caches are written no faster here
+// (93 us for a pass instead of 83): what reads them next then has to fetch them.
 template <typename TX, typename TR, typename TY, bool RES, int G, int NV>
 __global__ __launch_bounds__(G > 512 ? G : G > 64 ? 256 : 512,
                              G > 512 ? 4 : 2)
@@ -401,7 +400,9 @@ __global__ __launch_bounds__(1024) void ln_records_kernel(
 
 // ------------------------------------------------------------- long rows
 // A thread adds up a thousandth of the row: in fp64, for a chain of that many
-// float32 additions would be as far off as its length.
+// float32 additions would be as far off as its length. Three reads of the row,
+// by loads of one element: 512 x 20011 fp32 take 47 us forward, 48 backward and
+// 15 for the weights' records, where the bytes would take 12 and 18.
 constexpr int kLongThreads = 1024;
 
 template <typename TX, typename TR, bool RES>

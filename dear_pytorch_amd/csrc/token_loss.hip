@@ -529,13 +529,12 @@ __device__ __forceinline__ void put_top(const LogprobArgs& a, int64_t place,
 }
 
 // WHOLE: a slice is a whole row, and is finished here.
-// 4096 x 30528 bf16: 47 us without a top (5.3 TB/s), bound by memory and by the
-// vector unit alike, which is busy for three quarters of that: a conversion,
-// a subtraction, a product, exp2, two sums and the maximum for each element.
-// 68 us with a top of 32, where the phases of a block wait for each other, and
-// 107 with one of 128, 30 of it the ranking's reads of LDS. The row is never
-// read again from memory but for some hundred pieces that may hold one of the
-// top.
+// 4096 x 30528 bf16: 49 us without a top (5.1 TB/s), bound by memory and by the
+// vector unit alike, which is busy for 81 % of that: a conversion, a
+// subtraction, a product, exp2, two sums and the maximum for each element. 74 us
+// with a top of 32 (84 % busy), and 112 with one of 128, where the ranking reads
+// LDS for each pair. The row is never read again from memory but for some
+// hundred pieces that may hold one of the top.
 template <typename T, int NT, int NV, bool TOP, bool WHOLE>
 __global__ __launch_bounds__(NT, WHOLE ? 4 : 6) void logprobs_slice_kernel(
     const T* __restrict__ logits, const LogprobArgs a) {
@@ -596,7 +595,7 @@ __global__ __launch_bounds__(NT, WHOLE ? 4 : 6) void logprobs_slice_kernel(
 }
 
 // Four rows to a block, a wave each. Bound by the latency of its loads, one
-// after the other: 5 us of 4096 rows of one or two slices, 7 of 167 rows of
+// after the other: 5 us of 4096 rows of one or two slices, 6 of 167 rows of
 // four slices with a top of 20.
 template <typename T>
 __global__ __launch_bounds__(256) void logprobs_finish_kernel(
@@ -884,12 +883,12 @@ __device__ __forceinline__ void finish_distill(const DistillArgs& a,
           (float)(share * (x[e] * inv) - q[e]);
 }
 
-// 4096 x 30528 bf16, 32 entries, with the kernel that joins the slices: 48 us
-// without a tail; with one, where nothing is cached, 61 (4.1 TB/s). With a tail
-// the elements that are named have to be left out of maximum and sum exactly:
-// taking them from the sum afterwards, or summing the others relative to them,
-// would leave nothing of a small tail. They are known by a bit for each element
-// of a thread, which cost less than comparing the ids (67 us).
+// 4096 x 30528 bf16, 32 entries: 46 us without a tail (5.4 TB/s), 51 with one
+// (4.9 TB/s), and 9 for the kernel that joins the slices. With a tail the
+// elements that are named have to be left out of maximum and sum exactly: taking
+// them from the sum afterwards, or summing the others relative to them, would
+// leave nothing of a small tail. They are known by a bit for each element of a
+// thread, which cost less than comparing the ids (67 us).
 template <typename T, int NT, int NV, bool TAIL>
 __global__ __launch_bounds__(NT, 6) void distill_slice_kernel(
     const T* __restrict__ logits, const DistillArgs a) {
@@ -946,7 +945,7 @@ __global__ __launch_bounds__(NT, 6) void distill_slice_kernel(
 }
 
 // Four rows to a block, a wave each; N * 64 entries at most. Bound by latency,
-// of its loads and of fp64: 4 us of 614 rows, 7 of 4096.
+// of its loads and of fp64: 4 us of 614 rows, 9 of 4096.
 template <typename T, bool TAIL, int N>
 __global__ __launch_bounds__(256) void distill_finish_kernel(
     const T* __restrict__ logits, const DistillArgs a) {
@@ -977,7 +976,7 @@ __global__ __launch_bounds__(256) void distill_finish_kernel(
 // ----------------------------------------------------------------- backward
 // A block of 256 takes 512 vectors of one row. The last row comes first: what
 // the forward pass has read last is still in the last-level cache (4096 x 30528
-// bf16, 250 MB, in a pass of forward and backward: 88 us in the rows' order, 81
+// bf16, 250 MB, in a pass of forward and backward: 88 us in the rows' order, 80
 // in this one).
 constexpr int kBwdThreads = 256;
 constexpr int kBwdVectors = 2;
@@ -1032,7 +1031,7 @@ __device__ __forceinline__ void zero_piece(T* out, int len) {
 }
 
 // Bound by memory. 4096 x 30528 fp32 with 15 % of the rows labelled, 75 MB read
-// and 500 written: 85 us (6.8 TB/s); all labelled 157 us (6.4 TB/s). Rows that
+// and 500 written: 86 us (6.7 TB/s); all labelled 156 us (6.4 TB/s). Rows that
 // were not looked at are only written.
 template <typename T, bool ENT, bool STREAM>
 __global__ __launch_bounds__(kBwdThreads) void logprobs_bwd_kernel(
@@ -1102,8 +1101,8 @@ __global__ __launch_bounds__(kBwdThreads) void logprobs_bwd_kernel(
   }
 }
 
-// Bound by memory: 4096 x 30528 bf16, 81 us (6.2 TB/s); 614 rows of fp32,
-// 150 MB in all, 23.5 us (6.4 TB/s).
+// Bound by memory: 4096 x 30528 bf16, 80 us (6.2 TB/s); 614 rows of fp32,
+// 150 MB in all, 25 us (6.1 TB/s).
 template <typename T, bool STREAM>
 __global__ __launch_bounds__(kBwdThreads) void distill_bwd_kernel(
     const T* __restrict__ logits, int64_t zs,
@@ -1153,10 +1152,9 @@ Factor exp2_factor(double t) {
 // their phases better, larger ones leave fewer lists to make and join. Of 4096
 // and 2048 vectors, us: 614 of 4096 rows of 30528 fp32, no top, 28.8 and 25.0;
 // 4096 rows of 30528 bf16 with a top of 32 76.0 and 79.5, of 128 123 and 197;
-// distillation of the same with a tail 59.5 and 57.8, without 52.3 and 50.6.
-// Few rows, of 4096 and 1024 vectors: 1 x 131072 bf16, top 8, 12.7 and 11.9,
-// top 64 16.5 and 31.4; 2 x 600011 fp32, top 16, 15.7 and 20.5, top 128 46 and
-// 130.
+// distillation of the same without a tail 52.3 and 50.6. Few rows, of 4096 and
+// 1024 vectors: 1 x 131072 bf16, top 8, 12.7 and 11.9, top 64 16.5 and 31.4;
+// 2 x 600011 fp32, top 16, 15.7 and 20.5, top 128 46 and 130.
 struct Cut {
   int64_t each, slices;      // vectors of a slice, slices of a row
 };
