@@ -236,3 +236,12 @@ def test_gpu_a_tail_is_the_cpu_paths():
     for a, b, key in ((got, loss, "loss"), (dz, g, "dlogits")):
         check(a.cpu(), *want[key], what=key)
         check(b, *want[key], what=key)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])       # float16 ends at 65504
+@pytest.mark.parametrize("where", ["all", "last"])
+@pytest.mark.parametrize("V,K,T", [
+    (40, 3, 1e-4), (30528, 9, 1e-4), (40, 3, 1e4), (30528, 70, 1e4)])
+def test_gpu_far_at_the_ends_of_the_temperature(V, K, T, where, dtype):
+    far(V, K, T, dtype, "cuda", where)
